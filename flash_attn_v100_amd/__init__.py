@@ -43,10 +43,15 @@ HOT_PATH = (
     "forward_paged_decode_gqa_fp16", "forward_decode_int8_gqa",
 )
 
-for _name in API_NAMES:
+# Operators this build adds beside the reference's.
+ADDED_NAMES = (
+    "forward_scored", "forward_scored_with_lse", "backward_scored",
+)
+
+for _name in API_NAMES + ADDED_NAMES:
     globals()[_name] = getattr(_ext, _name)
 
-__all__ = list(API_NAMES)
+__all__ = list(API_NAMES + ADDED_NAMES)
 
 
 def library_path() -> str:

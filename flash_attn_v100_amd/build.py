@@ -29,7 +29,8 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
 
-KERNEL_SOURCES = ["decode.hip", "prefill.hip", "train.hip", "train_fp32.hip", "token_ops.hip", "tp_ops.hip"]
+KERNEL_SOURCES = ["decode.hip", "prefill.hip", "train.hip", "train_fp32.hip", "token_ops.hip", "tp_ops.hip",
+                  "scored.hip", "scored_fp32.hip"]
 HOST_SOURCES = ["capi.cpp"]
 
 HIP_FLAGS = [
@@ -44,7 +45,8 @@ HIP_FLAGS = [
 # 256 VGPRs hold, so they keep their accumulators (only ever accumulated and
 # stored) in AGPRs.
 VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-SOURCE_FLAGS = {"decode.hip": VGPR_FORM, "prefill.hip": VGPR_FORM, "train.hip": VGPR_FORM}
+SOURCE_FLAGS = {"decode.hip": VGPR_FORM, "prefill.hip": VGPR_FORM, "train.hip": VGPR_FORM,
+                "scored.hip": VGPR_FORM}
 
 
 def _run(cmd):

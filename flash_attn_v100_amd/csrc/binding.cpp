@@ -649,6 +649,119 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> backward(at::Tensor dout, at::Ten
   return std::make_tuple(dq, dk, dv);
 }
 
+// ---------------------------------------------------------------------------
+// Attention with modified scores: tanh cap, distance bias, document and prefix
+// masks (no counterpart in the reference).
+
+using OptTensor = c10::optional<at::Tensor>;
+
+// Checks an optional argument (given: of this type and shape, contiguous, on
+// q's device) and returns its pointer, nullptr if it is not given.
+template <typename T>
+const T* optional_ptr(const OptTensor& x, const at::Tensor& q, const char* name, at::ScalarType dtype,
+                      at::IntArrayRef sizes) {
+  if (!x.has_value()) return nullptr;
+  TORCH_CHECK(x->device() == q.device(), name, " must be on q's device");
+  TORCH_CHECK(x->is_contiguous(), name, " must be a contiguous tensor");
+  TORCH_CHECK(x->scalar_type() == dtype, name, " must be ", dtype == at::kInt ? "int32" : "float32");
+  TORCH_CHECK(x->sizes() == sizes, name, " must have shape ", sizes);
+  return x->data_ptr<T>();
+}
+
+void check_softcap(double softcap) {
+  const float cap = static_cast<float>(softcap);
+  TORCH_CHECK(cap == 0.0f || (cap >= 1e-3f && cap <= 1e6f), "softcap must be 0 (none) or lie in [1e-3, 1e6]");
+}
+
+struct ScoredArgs {
+  const float* slopes;
+  const int32_t* ids;
+  const int32_t* prefix;
+};
+
+ScoredArgs check_scored(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, bool causal, double softcap,
+                        const OptTensor& slopes, const OptTensor& doc_ids, const OptTensor& prefix_lens, bool training) {
+  CHECK_INPUT(q);
+  CHECK_INPUT(k);
+  CHECK_INPUT(v);
+  check_prefill_gqa_input_shapes(q, k, v);
+  TORCH_CHECK(q.dtype() == at::kHalf || q.dtype() == at::kFloat, "q, k, v must be float16 or float32");
+  const auto B = q.size(0), H_Q = q.size(1), N = q.size(2), D = q.size(3), H_KV = k.size(1);
+  TORCH_CHECK(H_KV > 0 && H_Q >= H_KV, "H_Q must be >= H_KV");
+  TORCH_CHECK(H_Q % H_KV == 0, "H_Q must be divisible by H_KV");
+  const bool narrow = training || q.dtype() == at::kFloat;
+  TORCH_CHECK(D <= (narrow ? kMaxD : kMaxDLarge),
+              narrow ? "D must be less than or equal to MAX_D(128)" : "D must be <= MAX_D_LARGE(256)");
+  check_softcap(softcap);
+  TORCH_CHECK(!prefix_lens.has_value() || causal, "prefix_lens needs causal=True");
+  return {optional_ptr<float>(slopes, q, "slopes", at::kFloat, {H_Q}),
+          optional_ptr<int32_t>(doc_ids, q, "doc_ids", at::kInt, {B, N}),
+          optional_ptr<int32_t>(prefix_lens, q, "prefix_lens", at::kInt, {B})};
+}
+
+std::tuple<at::Tensor, at::Tensor> scored_impl(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, bool causal,
+                                               double softcap, const OptTensor& slopes, const OptTensor& doc_ids,
+                                               const OptTensor& prefix_lens, bool want_lse) {
+  const ScoredArgs a = check_scored(q, k, v, causal, softcap, slopes, doc_ids, prefix_lens, want_lse);
+  HIPGuardMasqueradingAsCUDA guard(q.device());
+  auto out = at::empty_like(q);
+  at::Tensor lse;
+  if (want_lse) lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+  auto fn = q.dtype() == at::kHalf ? fa_scored_fp16 : fa_scored_fp32;
+  check_fa(fn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr,
+              to_int(q.size(0), "B"), to_int(q.size(1), "H_Q"), to_int(k.size(1), "H_KV"), to_int(q.size(2), "N"),
+              to_int(q.size(3), "D"), causal ? 1 : 0, static_cast<float>(softcap), a.slopes, a.ids, a.prefix,
+              cur_stream()));
+  return std::make_tuple(out, lse);
+}
+
+at::Tensor forward_scored(at::Tensor q, at::Tensor k, at::Tensor v, bool causal, double softcap, OptTensor slopes,
+                          OptTensor doc_ids, OptTensor prefix_lens) {
+  return std::get<0>(scored_impl(q, k, v, causal, softcap, slopes, doc_ids, prefix_lens, false));
+}
+
+std::tuple<at::Tensor, at::Tensor> forward_scored_with_lse(at::Tensor q, at::Tensor k, at::Tensor v, bool causal,
+                                                           double softcap, OptTensor slopes, OptTensor doc_ids,
+                                                           OptTensor prefix_lens) {
+  return scored_impl(q, k, v, causal, softcap, slopes, doc_ids, prefix_lens, true);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> backward_scored(at::Tensor dout, at::Tensor q, at::Tensor k, at::Tensor v,
+                                                               at::Tensor out, at::Tensor logsumexp, bool causal,
+                                                               double softcap, OptTensor slopes, OptTensor doc_ids,
+                                                               OptTensor prefix_lens) {
+  const ScoredArgs a = check_scored(q, k, v, causal, softcap, slopes, doc_ids, prefix_lens, true);
+  CHECK_INPUT(dout);
+  CHECK_INPUT(out);
+  CHECK_INPUT(logsumexp);
+  TORCH_CHECK(dout.sizes() == q.sizes(), "dout and q must have the same shape");
+  TORCH_CHECK(out.sizes() == q.sizes(), "out and q must have the same shape");
+  CHECK_SAME_DEVICE(dout, q);
+  CHECK_SAME_DEVICE(out, q);
+  CHECK_SAME_DEVICE(logsumexp, q);
+  CHECK_SAME_DTYPE(dout, q);
+  CHECK_SAME_DTYPE(out, q);
+  TORCH_CHECK(logsumexp.dtype() == at::kFloat, "logsumexp must be float32");
+  const auto B = q.size(0), H_Q = q.size(1), N = q.size(2), D = q.size(3);
+  CHECK_DIM(logsumexp, 3);
+  TORCH_CHECK(logsumexp.size(0) == B && logsumexp.size(1) == H_Q && logsumexp.size(2) == N,
+              "logsumexp shape must be [B, H_Q, N]");
+  HIPGuardMasqueradingAsCUDA guard(q.device());
+  auto dq = at::empty_like(q);
+  auto dk = at::empty_like(k);
+  auto dv = at::empty_like(v);
+  const int b = to_int(B, "B"), hq = to_int(H_Q, "H_Q"), hkv = to_int(k.size(1), "H_KV"), n = to_int(N, "N"),
+            d = to_int(D, "D");
+  const size_t bytes = fa_backward_workspace_size(b, hq, n);
+  at::Tensor ws;
+  if (bytes > 0) ws = at::empty({static_cast<int64_t>(bytes / sizeof(float))}, q.options().dtype(at::kFloat));
+  auto fn = q.dtype() == at::kHalf ? fa_scored_backward_fp16 : fa_scored_backward_fp32;
+  check_fa(fn(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), logsumexp.data_ptr<float>(),
+              dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), b, hq, hkv, n, d, causal ? 1 : 0, static_cast<float>(softcap),
+              a.slopes, a.ids, a.prefix, ws_ptr(ws), bytes, cur_stream()));
+  return std::make_tuple(dq, dk, dv);
+}
+
 // token_eviction (flash_attn_kernel.cu:4296-4344): (k_out, v_out, valid_mask).
 std::tuple<at::Tensor, at::Tensor, at::Tensor> token_eviction(at::Tensor k, at::Tensor v, at::Tensor attn_scores,
                                                               int num_evict) {
@@ -960,5 +1073,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cross_gpu_allreduce_fp16", &cross_gpu_allreduce_fp16, "fp16 dst += src on one device (MI355X)");
   m.def("scatter_heads", &scatter_heads, "Copy a head range of full into local (MI355X)");
   m.def("gather_heads", &gather_heads, "Copy local into a head range of full (MI355X)");
+  namespace py = pybind11;
+  m.def("forward_scored", &forward_scored, "Attention with capped, biased or masked scores (MI355X MFMA)", py::arg("q"),
+        py::arg("k"), py::arg("v"), py::arg("causal"), py::arg("softcap") = 0.0, py::arg("slopes") = py::none(),
+        py::arg("doc_ids") = py::none(), py::arg("prefix_lens") = py::none());
+  m.def("forward_scored_with_lse", &forward_scored_with_lse, "forward_scored with logsumexp (MI355X MFMA)", py::arg("q"),
+        py::arg("k"), py::arg("v"), py::arg("causal"), py::arg("softcap") = 0.0, py::arg("slopes") = py::none(),
+        py::arg("doc_ids") = py::none(), py::arg("prefix_lens") = py::none());
+  m.def("backward_scored", &backward_scored, "Backward of forward_scored_with_lse (MI355X MFMA)", py::arg("dout"),
+        py::arg("q"), py::arg("k"), py::arg("v"), py::arg("out"), py::arg("logsumexp"), py::arg("causal"),
+        py::arg("softcap") = 0.0, py::arg("slopes") = py::none(), py::arg("doc_ids") = py::none(),
+        py::arg("prefix_lens") = py::none());
   m.def("_fa_version", []() { return std::string(fa_version()); });
 }

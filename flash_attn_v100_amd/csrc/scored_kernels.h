@@ -1,0 +1,857 @@
+// Device kernels of attention with modified scores for gfx950: forward (with
+// optional log-sum-exp) and backward (dQ, dK, dV), fp16 and fp32, grouped KV
+// heads.  Instantiated by scored.hip (fp16) and scored_fp32.hip.
+//
+//   s_ij   = q_i . k_j / sqrt(D)
+//   c_ij   = cap tanh(s_ij / cap)            (cap > 0; else s_ij)
+//   y_ij   = c_ij - slope_h |i - j|
+//   j is visible to i iff (no ids, or id_i = id_j >= 0) and
+//                         (not causal, or j <= i, or j < prefix_b)
+//   P_ij   = exp(y_ij - lse_i) over the visible j, O_i = sum_j P_ij V_j
+//   dY_ij  = P_ij (dO_i . V_j - delta_i), delta_i = sum_d dO_id O_id
+//   dS_ij  = dY_ij (1 - (c_ij / cap)^2)
+//   dQ = dS K / sqrt(D), dK = dS^T Q / sqrt(D), dV = P^T dO (dK, dV summed over
+//   the query heads of the KV head)
+// A row that sees nothing has O = 0, lse = -inf and takes no part in the
+// gradients.  Rows of negative id are padding: whatever they hold, NaN
+// included, reaches no other row (their staged tile rows are zeroed).
+//
+// Shapes, operand layouts and tile streaming are the training kernels'
+// (train_tiles.h): 4 waves of 32 rows, 32-row tiles through a two-stage LDS
+// ring, S^T = K Q^T with one query per lane (query-major: forward, dQ), S = Q
+// K^T with one key per lane (key-major: dK, dV).  A KV head's query heads are
+// streamed in turn past the key-major kernel's keys, so dK and dV add up in
+// registers in a fixed order, without atomics.
+//
+// Document masks: a workgroup walks only the tiles that hold an id in the range of its
+// own rows' ids.  Every 64 sub-tiles of 32 rows each lane reads one
+// sub-tile's ids (8 16-byte loads) and keeps its range; the live ones
+// are a 64-bit ballot that scalar code steps through.  A sub-tile of a single id needs no
+// per-element mask where the wave's rows hold that id too; the others compare
+// ids element by element.
+#pragma once
+
+#include "train_tiles.h"
+
+namespace fa {
+namespace scored {
+
+using train::acc_frag;
+using train::Elem;
+using train::kBlockRows;
+using train::kLn2;
+using train::kRows;
+using train::kThreads;
+using train::kWaves;
+using train::Layout;
+using train::lds_ptr;
+using train::load_frag;
+using train::mma;
+using train::part_slot;
+using train::Reader;
+using train::TileRing;
+using train::zero_frag;
+
+// What a kernel variant applies to the scores; kAnyMods reads it from the
+// call's parameters instead (uniform branches).
+enum Mods : int { kCap = 1, kBias = 2, kDocs = 4, kAnyMods = 8 };
+
+struct ScoredParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* o;          // backward: forward output
+  const void* dout;       // backward
+  void* out;              // forward: O; backward: dQ
+  void* dk;
+  void* dv;
+  float* lse;             // forward: written if non-null; backward: read
+  float* delta;           // backward workspace [B * H_Q * N]
+  const float* slopes;    // [H_Q] or null
+  const int32_t* ids;     // [B, N] or null
+  const int32_t* prefix;  // [B] or null (causal only)
+  int mods;
+  int B, H_Q, H_KV, N, D, G, causal;
+  int nblk;               // row blocks (one workgroup each) per head
+  int heads;              // query heads dealt with one unit (query-major)
+  int units, group_units; // units of the grid, and how many an XCD interleaves
+  float scale;            // 1/sqrt(D)
+  float scale_log2;       // scale * log2(e)
+  float cap_in;           // scale / cap
+  float cap_log2;         // cap * log2(e)
+};
+
+template <int MODS>
+__device__ __forceinline__ bool has(const ScoredParams& p, int m) {
+  if constexpr ((MODS & kAnyMods) != 0) return (p.mods & m) != 0;
+  return (MODS & m) != 0;
+}
+
+constexpr int kXcds = 8;
+
+// Workgroup -> (unit u, head of the unit, row block).  Units are dealt to the
+// XCDs round-robin (the dispatcher sends workgroup j to XCD j % 8), an XCD
+// interleaves group_units of them, heaviest block first, so the blocks that
+// stream the same tiles run together behind one L2.  Returns false for the
+// padding workgroups of the last round.  group_units 0: block by block, all
+// heads' heaviest first.
+__device__ __forceinline__ bool map_block(const ScoredParams& p, int heads, bool heavy_last, int& u, int& head, int& blk) {
+  const int j = static_cast<int>(blockIdx.x);
+  if (p.group_units == 0) {
+    const int pair = j % (p.units * heads), b = j / (p.units * heads);
+    u = pair / heads;
+    head = pair % heads;
+    blk = heavy_last ? p.nblk - 1 - b : b;
+    return true;
+  }
+  const int i = j / kXcds;
+  const int per_row = p.group_units * heads;
+  const int group = i / (per_row * p.nblk);
+  const int ii = i % (per_row * p.nblk);
+  const int b = ii / per_row;
+  const int hg = ii % per_row;
+  u = j % kXcds + kXcds * (group * p.group_units + hg / heads);
+  head = hg % heads;
+  blk = heavy_last ? p.nblk - 1 - b : b;
+  return u < p.units;
+}
+
+typedef int int4u __attribute__((ext_vector_type(4), aligned(4)));
+
+__device__ __forceinline__ int wave_min_i(int x) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) x = min(x, __shfl_xor(x, off, 64));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ int wave_max_i(int x) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) x = max(x, __shfl_xor(x, off, 64));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
+constexpr int kMixedIds = -1;       // a sub-tile of several ids (or a ragged one)
+constexpr int kNoId = -2147483647;  // own rows that see nothing; differs from every staged id
+
+// The tiles a workgroup streams: SUBS 32-row sub-tiles each, `count` of them
+// from row `first`, last to first with `rev`.  With ids, only those that hold
+// an id of [lo, hi].
+template <int SUBS>
+struct TileWalk {
+  const int32_t* ids;  // of the streamed rows' batch row, or null
+  int rows, first, count, lo, hi;
+  bool rev;
+  int vt = 0;          // without ids: next tile in walk order
+  int base = -64;      // with ids: first sub-tile (in walk order) of the group held
+  uint64_t live = 0, pads = 0;
+  int uni = 0;         // this lane's sub-tile: its single id, or kMixedIds
+  // the tile that next() gave
+  int tile = -1;
+  uint64_t cur_pads = 0;
+
+  __device__ __forceinline__ void scan() {
+    const int lane = threadIdx.x & 63;
+    const int v = base + lane;
+    const int t = v / SUBS;
+    int mn = 0x7fffffff, mx = -1;
+    bool pad = false, ragged = true;
+    if (t < count) {
+      const int r0 = first + ((rev ? count - 1 - t : t) * SUBS + v % SUBS) * kRows;
+      ragged = r0 + kRows > rows;
+      auto take = [&](int id) {
+        pad |= id < 0;
+        if (id >= 0) mn = min(mn, id);
+        mx = max(mx, id);
+      };
+      if (!ragged) {
+        int4u x[kRows / 4];
+#pragma unroll
+        for (int i = 0; i < kRows / 4; ++i) x[i] = *reinterpret_cast<const int4u*>(ids + r0 + 4 * i);
+#pragma unroll
+        for (int i = 0; i < kRows / 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) take(x[i][j]);
+      } else {
+        for (int r = r0; r < rows; ++r) take(ids[r]);
+      }
+    }
+    uni = !ragged && !pad && mn == mx ? mn : kMixedIds;
+    live = __builtin_amdgcn_ballot_w64(mx >= lo && mn <= hi && mn <= mx);
+    pads = __builtin_amdgcn_ballot_w64(pad);
+  }
+  // Steps to the next tile; false when there is none.  Every lane of every
+  // wave of the workgroup takes the same steps.
+  __device__ __forceinline__ bool next() {
+    if (ids == nullptr) {
+      if (vt >= count) return false;
+      tile = rev ? count - 1 - vt : vt;
+      ++vt;
+      return true;
+    }
+    while (live == 0) {
+      base += 64;
+      if (base >= count * SUBS) return false;
+      scan();
+    }
+    const int bit = __builtin_ctzll(live) / SUBS * SUBS;
+    const uint64_t mask = (SUBS == 1 ? 1ull : (1ull << SUBS) - 1) << bit;
+    live &= ~mask;
+    cur_pads = pads & mask;
+    const int v = (base + bit) / SUBS;
+    tile = rev ? count - 1 - v : v;
+    at = bit;
+    return true;
+  }
+  int at = 0;
+  // Single id of sub-tile `sub` of the current tile, or kMixedIds.
+  __device__ __forceinline__ int sub_id(int sub) const { return __builtin_amdgcn_readlane(uni, at + sub); }
+};
+
+// ---- scores ----
+// tanh z = z (1 + w P(w)), w = z^2, for |z| <= 1/2: P fitted to the least
+// largest relative error (1.5e-8; 7.4e-8 evaluated in fp32).
+constexpr float kTanhMax = 0.5f;
+constexpr float kT0 = -0.333331435918808f, kT1 = 0.13325878977775574f, kT2 = -0.05304547771811485f,
+                kT3 = 0.01724146120250225f;
+
+// Raw products s -> capped scores in the log2 domain, cap log2(e) tanh(s scale / cap).
+// Where every |z| of the wave's tile is at most 1/2 (scores below half the
+// cap) the polynomial serves: 8 full-rate operations a score where the
+// exponential form needs two quarter-rate ones more.
+__device__ __forceinline__ void cap_scores(float16_t& s, const ScoredParams& p) {
+  float16_t z;
+  float big = 0.0f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    z[r] = s[r] * p.cap_in;
+    big = fmaxf(big, fabsf(z[r]));
+  }
+  const bool far = __builtin_amdgcn_ballot_w64(!(big <= kTanhMax)) != 0;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const float w = z[r] * z[r];
+    const float pw = fmaf(fmaf(fmaf(kT3, w, kT2), w, kT1), w, kT0);
+    const float zc = z[r] * p.cap_log2;
+    s[r] = fmaf(zc * w, pw, zc);
+  }
+  if (far) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      // 1 - 2 / (e^2|z| + 1): at least 0.46 here, so nothing cancels
+      const float e = fast_exp2(fabsf(z[r]) * (2.0f * kLog2e));
+      const float t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
+      const float y = __builtin_copysignf(t * p.cap_log2, z[r]);
+      s[r] = fabsf(z[r]) <= kTanhMax ? s[r] : y;
+      // (NaN compares false and comes through the exponential)
+    }
+  }
+}
+
+// Distances of a tile's elements: element r lies `rel` + 8 (r / 4) + r % 4 from the lane's row.
+__device__ __forceinline__ void add_bias(float16_t& y, float slope2, float rel) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) y[r] = fmaf(-slope2, fabsf(rel + static_cast<float>(8 * (r >> 2) + (r & 3))), y[r]);
+}
+
+// Ids of the 16 tile rows r0 + 8 (r / 4) + r % 4 (negative ones as -1), -1 past `rows`.
+__device__ __forceinline__ void load_ids(int (&id)[16], const int32_t* ids, int r0, int rows) {
+#pragma unroll
+  for (int rr = 0; rr < 4; ++rr) {
+    const int row = r0 + 8 * rr;
+    if (row + 4 <= rows) {
+      const int4u x = *reinterpret_cast<const int4u*>(ids + row);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) id[4 * rr + j] = max(x[j], -1);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) id[4 * rr + j] = row + j < rows ? max(ids[row + j], -1) : -1;
+    }
+  }
+}
+
+// Zeroes the rows of negative id in the staged tile pair of rows [r0, r0 + SR)
+// (rows past `rows` may hold the last one again).
+template <typename T, typename Ring>
+__device__ __forceinline__ void zero_pad_rows(const Ring& ring, int stage, const int32_t* ids, int r0, int rows) {
+  lds_ptr<T> ta = ring.tile_a(stage);
+  lds_ptr<T> tb = ring.tile_b(stage);
+  typedef typename Elem<T>::frag F;
+  for (int c = threadIdx.x; c < Ring::CHUNKS; c += kThreads) {
+    const int row = c / Ring::CPR, col = c % Ring::CPR * 8;
+    if (ids[min(r0 + row, rows - 1)] < 0) {
+      *reinterpret_cast<__attribute__((address_space(3))) F*>(ta + Ring::L::off(row, col)) = zero_frag<T>();
+      *reinterpret_cast<__attribute__((address_space(3))) F*>(tb + Ring::L::off(row, col)) = zero_frag<T>();
+    }
+  }
+}
+
+// Streams the walk's tiles through the ring, HEADS rounds a tile (key-major:
+// the query heads in turn), and calls compute(stage, tile, round, sub id) for
+// each; fetch(tile, round, stage) copies (DMA) or loads (registers) one.
+template <typename T, typename Ring, bool DMA, int SUBS, typename Fetch, typename Compute>
+__device__ __forceinline__ void stream_tiles(Ring& ring, TileWalk<SUBS>& walk, int heads, int sub, int N, Fetch&& fetch,
+                                             Compute&& compute) {
+  bool more = walk.next();
+  if (!more) return;
+  int tile = walk.tile, id = walk.ids ? walk.sub_id(sub) : 0, head = 0, stage = 0;
+  uint64_t pads = walk.cur_pads;
+  fetch(tile, 0, 0);
+  if constexpr (!DMA) ring.store(0);
+  for (;;) {
+    // the (tile, head) after this one
+    int ntile = tile, nid = id, nhead = head + 1;
+    uint64_t npads = pads;
+    if (nhead == heads) {
+      nhead = 0;
+      more = walk.next();
+      ntile = walk.tile;
+      npads = walk.cur_pads;
+      if (walk.ids && more) nid = walk.sub_id(sub);
+    }
+    if constexpr (DMA) {
+      ring.wait_dma(false);  // this wave's copies of the tile have landed
+      tile_barrier();        // everyone's have; the other stage is free
+    } else {
+      __syncthreads();
+    }
+    if (pads != 0) {
+      zero_pad_rows<T>(ring, stage, walk.ids, walk.first + tile * SUBS * kRows, N);
+      __syncthreads();
+    }
+    if (more) fetch(ntile, nhead, stage ^ 1);
+    compute(stage, tile, head, id);
+    if (!more) break;
+    if constexpr (!DMA) ring.store(stage ^ 1);
+    tile = ntile;
+    id = nid;
+    head = nhead;
+    pads = npads;
+    stage ^= 1;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Query-major kernel: MODE 0 = forward (O, optional LSE), MODE 1 = dQ + delta.
+template <typename T, int DP, int DC, int ROWS, int MODE, int SPLIT, int MODS>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP <= 64 ? 2 : 1))) void scored_query_kernel(
+    ScoredParams p) {
+  typedef typename Elem<T>::frag F;
+  constexpr int KK = DC / 16;
+  constexpr int DB = (DC + 31) / 32;
+  constexpr bool DMA = ROWS != kRowElems && sizeof(T) == 2;
+  constexpr int RW = kWaves / SPLIT;  // 32-row blocks per workgroup
+  typedef TileRing<T, DP, DMA, false, kRows * SPLIT, ROWS> Ring;
+  __shared__ __attribute__((aligned(1024))) char smem[Ring::BYTES];
+
+  const int N = p.N, D = p.D;
+  int u, hg, blk;
+  if (!map_block(p, p.heads, p.causal != 0, u, hg, blk)) return;
+  const int units_per_b = p.H_Q / p.heads;
+  const int b = u / units_per_b;
+  const int h = u % units_per_b * p.heads + hg;
+  const int hk = h / p.G;
+  const int q0 = blk * (RW * kRows);
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31;
+  const int hi = lane >> 5;
+  const int sub = wave / RW;
+  const int wq0 = q0 + (wave % RW) * kRows;
+  const int qrow = wq0 + l32;
+  const size_t qhead = static_cast<size_t>(b) * p.H_Q + h;
+  const size_t qbase = qhead * N * D;
+  const size_t kbase = (static_cast<size_t>(b) * p.H_KV + hk) * N * D;
+  const T* __restrict__ kp = static_cast<const T*>(p.k) + kbase;
+  const T* __restrict__ vp = static_cast<const T*>(p.v) + kbase;
+  const bool cap = has<MODS>(p, kCap), bias = has<MODS>(p, kBias), docs = has<MODS>(p, kDocs);
+
+  TileWalk<SPLIT> walk;
+  walk.ids = docs ? p.ids + static_cast<size_t>(b) * N : nullptr;
+  int my_id = 0, wlo = 0, whi = 0;
+  if (docs) {
+    my_id = qrow < N ? walk.ids[qrow] : -1;
+    my_id = my_id < 0 ? kNoId : my_id;
+    wlo = wave_min_i(my_id < 0 ? 0x7fffffff : my_id);
+    whi = wave_max_i(my_id);
+    int lo = 0x7fffffff, hi_ = -1;
+    for (int r = lane; r < RW * kRows; r += 64) {
+      const int id = q0 + r < N ? walk.ids[q0 + r] : -1;
+      if (id >= 0) lo = min(lo, id);
+      hi_ = max(hi_, id);
+    }
+    walk.lo = wave_min_i(lo);
+    walk.hi = wave_max_i(hi_);
+  }
+  const bool live = qrow < N && my_id >= 0;  // this lane's row sees something
+  // single id of the wave's rows, or none
+  const int wid = docs && wlo == whi && __builtin_amdgcn_ballot_w64(my_id != whi) == 0 ? whi : kNoId;
+
+  // resident B operands: lane's query row, d = 16 kk + 8 hi .. +8
+  F qf[KK], df[KK];
+  float delta = 0.0f, lse2 = 0.0f;
+  {
+    const T* qr = static_cast<const T*>(p.q) + qbase + static_cast<size_t>(min(qrow, N - 1)) * D;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) qf[kk] = live ? load_frag<T, ROWS>(qr, 16 * kk + 8 * hi, D) : zero_frag<T>();
+  }
+  if constexpr (MODE == 1) {
+    const size_t row = qbase + static_cast<size_t>(min(qrow, N - 1)) * D;
+    const T* dr = static_cast<const T*>(p.dout) + row;
+    const T* orow = static_cast<const T*>(p.o) + row;
+    float part = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      df[kk] = live ? load_frag<T, ROWS>(dr, 16 * kk + 8 * hi, D) : zero_frag<T>();
+      const F of = live ? load_frag<T, ROWS>(orow, 16 * kk + 8 * hi, D) : zero_frag<T>();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part = fmaf(static_cast<float>(df[kk][j]), static_cast<float>(of[j]), part);
+    }
+    delta = part + __shfl_xor(part, 32, 64);
+    if (qrow < N && hi == 0 && sub == 0) p.delta[qhead * N + qrow] = delta;
+    lse2 = live ? p.lse[qhead * N + qrow] * kLog2e : INFINITY;
+    if (lse2 == -INFINITY) lse2 = INFINITY;  // rows that see nothing: P = 0
+  }
+
+  float16_t acc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[db][r] = 0.0f;
+  float m_run = kNegBig, l_run = 0.0f;  // forward only (log2 domain)
+  const float c = cap || bias ? 1.0f : p.scale_log2;
+  const float slope2 = bias ? p.slopes[h] * kLog2e : 0.0f;
+
+  // keys every row sees, and the last key of this lane's row
+  const int pre = p.prefix != nullptr ? max(0, min(p.prefix[b], N)) : 0;
+  const int last = p.causal ? max(min(qrow, N - 1), pre - 1) : N - 1;
+  const int kend = p.causal ? max(min(N, q0 + RW * kRows), pre) : N;
+  const int kend_w = wq0 >= N ? 0 : (p.causal ? max(min(N, wq0 + kRows), pre) : N);
+  constexpr int SR = Ring::SR;
+  walk.rows = N;
+  walk.first = 0;
+  walk.count = (kend + SR - 1) / SR;
+  // With a bias the nearest keys weigh most: a causal walk that starts at the
+  // diagonal finds the running maximum at once.
+  walk.rev = bias && p.causal;
+
+  Ring ring(smem, tid, D);
+  const Reader<T, DP> rd(lane);
+  constexpr unsigned kSubBytes = kRows * Layout<T, DP>::LD * sizeof(T);
+  auto fetch = [&](int tile, int, int stage) {
+    if constexpr (DMA) ring.dma(kp, vp, nullptr, nullptr, tile * SR, N, D, stage);
+    else ring.load(kp, vp, nullptr, nullptr, tile * SR, N, D);
+  };
+  stream_tiles<T, Ring, DMA, SPLIT>(ring, walk, 1, sub, N, fetch, [&](int stage, int tile, int, int id) {
+    const int kt = tile * SR + sub * kRows;
+    if (kt >= kend_w) return;                               // past this wave's rows
+    if (docs && id >= 0 && (id < wlo || id > whi)) return;  // a document of other waves' rows
+    const unsigned ks = ring.addr_a(stage) + sub * kSubBytes;
+    const unsigned vs = ring.addr_b(stage) + sub * kSubBytes;
+    // S^T = K Q^T: lane <-> query, register r <-> key kt + 8 (r/4) + 4 hi + r%4
+    float16_t s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) s = mma(rd.row(ks, kk), qf[kk], s);
+    if (cap) {
+      cap_scores(s, p);
+    } else if (bias) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] *= p.scale_log2;
+    }
+    float16_t dt;  // dQ: derivative of the cap
+    if constexpr (MODE == 1) {
+      if (cap) {
+        const float inv = 1.0f / p.cap_log2;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float t = s[r] * inv;
+          dt[r] = fmaf(-t, t, 1.0f);
+        }
+      }
+    }
+    if (bias) add_bias(s, slope2, static_cast<float>(kt + 4 * hi - qrow));
+    if (kt + kRows > N || (p.causal && kt + kRows - 1 > max(wq0, pre - 1))) {
+      const int bound = last - kt - 4 * hi;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) > bound ? -INFINITY : s[r];
+    }
+    if (docs && (id < 0 || id != wid)) {
+      if (id >= 0) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = my_id == id ? s[r] : -INFINITY;
+      } else {
+        int key_id[16];
+        load_ids(key_id, walk.ids, kt + 4 * hi, N);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = my_id == key_id[r] ? s[r] : -INFINITY;
+      }
+    }
+    float16_t pm;  // P^T (forward) or dS^T (dQ)
+    if constexpr (MODE == 0) {
+      // p = exp2(s c - m) against the running max m, which is only refreshed
+      // (and O, l rescaled) when a lane's partial sum passes 2^8, i.e. some
+      // score outgrew m by more than the slack (always so from m = -1e30).
+      constexpr float kRescaleLimit = 256.0f;
+      float ls = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        pm[r] = fast_exp2(fmaf(s[r], c, -m_run));
+        ls += pm[r];
+      }
+      if (__builtin_amdgcn_ballot_w64(!(ls <= kRescaleLimit)) != 0) {
+        float mx = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+        const float mn = fmaxf(m_run, mx);
+        const float alpha = fast_exp2(m_run - mn);
+        m_run = mn;
+        l_run *= alpha;
+        ls = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          pm[r] = fast_exp2(fmaf(s[r], c, -mn));
+          ls += pm[r];
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
+      }
+      l_run += ls;
+    } else {
+      // dP^T = V dO^T
+      float16_t dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) dp = mma(rd.row(vs, kk), df[kk], dp);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) pm[r] = fast_exp2(fmaf(s[r], c, -lse2)) * (dp[r] - delta);
+      if (cap) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) pm[r] *= dt[r];
+      }
+    }
+    const F pf0 = acc_frag<T>(pm, 0), pf1 = acc_frag<T>(pm, 1);
+    // forward: O^T += V^T P^T;  dQ: dQ^T += K^T dS^T
+    const unsigned src = (MODE == 0) ? vs : ks;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      acc[db] = mma(rd.tr(src, 0, db), pf0, acc[db]);
+      acc[db] = mma(rd.tr(src, 16, db), pf1, acc[db]);
+    }
+  });
+
+  // ---- join the row block's waves: wave `sub` 0 takes the others' partials ----
+  if constexpr (SPLIT > 1) {
+    constexpr int REGS = 16 * DB + (MODE == 0 ? 2 : 0);
+    static_assert((SPLIT - 1) * RW * REGS * 256 <= Ring::BYTES, "partials fit the ring");
+    __syncthreads();  // every wave is done reading the ring
+    if (sub > 0) {
+      lds_ptr<float> out = part_slot<REGS>(smem, wave - RW, lane);
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) out[(16 * db + r) * 64] = acc[db][r];
+      if constexpr (MODE == 0) {
+        out[16 * DB * 64] = m_run;
+        out[(16 * DB + 1) * 64] = l_run;
+      }
+    }
+    __syncthreads();
+    if (sub > 0) return;
+    // a wave that saw no key has m = -1e30, l = 0 and weighs nothing
+#pragma unroll
+    for (int w = 0; w < SPLIT - 1; ++w) {
+      lds_ptr<float> in = part_slot<REGS>(smem, w * RW + wave, lane);
+      float a0 = 1.0f, a1 = 1.0f;
+      if constexpr (MODE == 0) {
+        const float m1 = in[16 * DB * 64];
+        const float mn = fmaxf(m_run, m1);
+        a0 = fast_exp2(m_run - mn);
+        a1 = fast_exp2(m1 - mn);
+        m_run = mn;
+        l_run = l_run * a0 + in[(16 * DB + 1) * 64] * a1;
+      }
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          acc[db][r] = MODE == 0 ? acc[db][r] * a0 + in[(16 * db + r) * 64] * a1 : acc[db][r] + in[(16 * db + r) * 64];
+    }
+  }
+
+  // ---- store: lane's row, d = 32 db + 8 (r/4) + 4 hi + r%4 ----
+  float mul;
+  if constexpr (MODE == 0) {
+    const float lt = l_run + __shfl_xor(l_run, 32, 64);
+    mul = !live || lt == 0.0f ? 0.0f : 1.0f / lt;
+    if (p.lse != nullptr && qrow < N && hi == 0)
+      p.lse[qhead * N + qrow] = !live || lt == 0.0f ? -INFINITY : (m_run + log2f(lt)) * kLn2;
+  } else {
+    mul = p.scale;
+  }
+  if (qrow >= N) return;
+  T* op = static_cast<T*>(p.out) + qbase + static_cast<size_t>(qrow) * D;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int rr = 0; rr < 4; ++rr) {
+      const int d0 = 32 * db + 8 * rr + 4 * hi;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (ROWS == kRowFull || d0 + j < D) op[d0 + j] = static_cast<T>(live ? acc[db][4 * rr + j] * mul : 0.0f);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Key-major kernel for 32 keys per wave: PASS 0 = dV, 1 = dK, 2 = both.
+constexpr int kPassDV = 0, kPassDK = 1, kPassBoth = 2;
+template <typename T, int DP, int DC, int ROWS, int PASS, int SPLIT, int MODS>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP <= 64 ? 2 : 1))) void scored_key_kernel(
+    ScoredParams p) {
+  constexpr bool DO_DV = PASS != kPassDK;
+  constexpr bool DO_DK = PASS != kPassDV;
+  typedef typename Elem<T>::frag F;
+  constexpr int KK = DC / 16;
+  constexpr int DB = (DC + 31) / 32;
+  constexpr bool DMA = ROWS != kRowElems && sizeof(T) == 2;
+  constexpr int RW = kWaves / SPLIT;  // 32-key blocks per workgroup
+  typedef TileRing<T, DP, DMA, true, kRows * SPLIT, ROWS> Ring;
+  __shared__ __attribute__((aligned(1024))) char smem[Ring::BYTES];
+
+  const int N = p.N, D = p.D;
+  int u, hg, blk;
+  if (!map_block(p, 1, false, u, hg, blk)) return;
+  const int b = u / p.H_KV, hk = u % p.H_KV;
+  const int k0 = blk * (RW * kRows);
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31;
+  const int hi = lane >> 5;
+  const int sub = wave / RW;
+  const int wk0 = k0 + (wave % RW) * kRows;
+  const int krow = wk0 + l32;
+  const size_t kbase = (static_cast<size_t>(b) * p.H_KV + hk) * N * D;
+  const size_t qhead0 = static_cast<size_t>(b) * p.H_Q + static_cast<size_t>(hk) * p.G;  // first query head of the group
+  const bool cap = has<MODS>(p, kCap), bias = has<MODS>(p, kBias), docs = has<MODS>(p, kDocs);
+
+  TileWalk<SPLIT> walk;
+  walk.ids = docs ? p.ids + static_cast<size_t>(b) * N : nullptr;
+  int my_id = 0, wlo = 0, whi = 0;
+  if (docs) {
+    my_id = krow < N ? walk.ids[krow] : -1;
+    my_id = my_id < 0 ? kNoId : my_id;
+    wlo = wave_min_i(my_id < 0 ? 0x7fffffff : my_id);
+    whi = wave_max_i(my_id);
+    int lo = 0x7fffffff, hi_ = -1;
+    for (int r = lane; r < RW * kRows; r += 64) {
+      const int id = k0 + r < N ? walk.ids[k0 + r] : -1;
+      if (id >= 0) lo = min(lo, id);
+      hi_ = max(hi_, id);
+    }
+    walk.lo = wave_min_i(lo);
+    walk.hi = wave_max_i(hi_);
+  }
+  const bool live = krow < N && my_id >= 0;
+  const int wid = docs && wlo == whi && __builtin_amdgcn_ballot_w64(my_id != whi) == 0 ? whi : kNoId;
+
+  F kf[KK], vf[KK];
+  {
+    const size_t row = kbase + static_cast<size_t>(min(krow, N - 1)) * D;
+    const T* kr = static_cast<const T*>(p.k) + row;
+    const T* vr = static_cast<const T*>(p.v) + row;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      kf[kk] = live ? load_frag<T, ROWS>(kr, 16 * kk + 8 * hi, D) : zero_frag<T>();
+      if constexpr (DO_DK) vf[kk] = live ? load_frag<T, ROWS>(vr, 16 * kk + 8 * hi, D) : zero_frag<T>();
+    }
+  }
+  float16_t dk[DB], dv[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      dk[db][r] = 0.0f;
+      dv[db][r] = 0.0f;
+    }
+  const float c = cap || bias ? 1.0f : p.scale_log2;
+  const int pre = p.prefix != nullptr ? max(0, min(p.prefix[b], N)) : 0;
+  // causal: rows before the first key see it only inside the prefix
+  const int qstart = p.causal && k0 >= pre ? k0 : 0;
+  constexpr int SR = Ring::SR;
+  walk.rows = N;
+  walk.first = qstart;
+  walk.count = (N - qstart + SR - 1) / SR;
+  // causal blocks of a head all end at the last query tile: walking backwards
+  // they read each tile at about the same time and share it through L2
+  walk.rev = p.causal != 0 && !docs;
+  const bool every = !p.causal || wk0 + kRows <= pre;  // every query sees the wave's keys
+  const int key_from = p.causal && krow >= pre ? krow : 0;
+
+  Ring ring(smem, tid, D);
+  const Reader<T, DP> rd(lane);
+  constexpr unsigned kSubBytes = kRows * Layout<T, DP>::LD * sizeof(T);
+  auto fetch = [&](int tile, int g, int stage) {
+    const size_t head = qhead0 + g;
+    const T* qp = static_cast<const T*>(p.q) + head * N * D;
+    const T* dp = static_cast<const T*>(p.dout) + head * N * D;
+    const float* lse = p.lse + head * N;
+    // the dV pass never reads delta: lse stands in for it in its stream
+    const float* second = DO_DK ? p.delta + head * N : lse;
+    if constexpr (DMA) ring.dma(qp, dp, lse, second, qstart + tile * SR, N, D, stage);
+    else ring.load(qp, dp, lse, second, qstart + tile * SR, N, D);
+  };
+  stream_tiles<T, Ring, DMA, SPLIT>(ring, walk, p.G, sub, N, fetch, [&](int stage, int tile, int g, int id) {
+    const int qt = qstart + tile * SR + sub * kRows;
+    if (qt >= N || wk0 >= N) return;
+    if (!every && wk0 >= pre && qt + kRows <= wk0) return;  // rows before every key of the wave
+    if (docs && id >= 0 && (id < wlo || id > whi)) return;
+    const unsigned qs = ring.addr_a(stage) + sub * kSubBytes;
+    const unsigned ds = ring.addr_b(stage) + sub * kSubBytes;
+    // S = Q K^T and dP = dO V^T: lane <-> key, register r <-> query qt + 8 (r/4) + 4 hi + r%4
+    float16_t s, dp;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] = 0.0f;
+      dp[r] = 0.0f;
+    }
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      s = mma(rd.row(qs, kk), kf[kk], s);
+      if constexpr (DO_DK) dp = mma(rd.row(ds, kk), vf[kk], dp);
+    }
+    if (cap) {
+      cap_scores(s, p);
+    } else if (bias) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] *= p.scale_log2;
+    }
+    float16_t dt;
+    if constexpr (DO_DK) {
+      if (cap) {
+        const float inv = 1.0f / p.cap_log2;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float t = s[r] * inv;
+          dt[r] = fmaf(-t, t, 1.0f);
+        }
+      }
+    }
+    if (bias) add_bias(s, p.slopes[hk * p.G + g] * kLog2e, static_cast<float>(qt + 4 * hi - krow));
+    const __attribute__((address_space(3))) float* lv = ring.vec(stage, 0) + sub * kRows;
+    const __attribute__((address_space(3))) float* dvv = ring.vec(stage, 1) + sub * kRows;
+    const float lmul = DMA ? kLog2e : 1.0f;  // the register path stores lse pre-scaled
+    float16_t pm, dsm;
+#pragma unroll
+    for (int rr = 0; rr < 4; ++rr) {
+      const float4_t l4 = *reinterpret_cast<const __attribute__((address_space(3))) float4_t*>(lv + 8 * rr + 4 * hi);
+      float4_t d4;
+      if constexpr (DO_DK) d4 = *reinterpret_cast<const __attribute__((address_space(3))) float4_t*>(dvv + 8 * rr + 4 * hi);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * rr + j;
+        pm[r] = fast_exp2(fmaf(s[r], c, -l4[j] * lmul));
+        if constexpr (DO_DK) dsm[r] = (dp[r] - d4[j]) * pm[r];
+      }
+    }
+    if constexpr (DO_DK) {
+      if (cap) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dsm[r] *= dt[r];
+      }
+    }
+    // masks select, since a masked element may be infinite or NaN
+    auto keep = [&](int r, bool ok) {
+      pm[r] = ok ? pm[r] : 0.0f;
+      if constexpr (DO_DK) dsm[r] = ok ? dsm[r] : 0.0f;
+    };
+    if (qt + kRows > N || (!every && qt < wk0 + kRows - 1)) {
+      const int from = key_from - qt - 4 * hi, lim = N - qt - 4 * hi;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int rel = 8 * (r >> 2) + (r & 3);
+        keep(r, rel >= from && rel < lim);
+      }
+    }
+    if (docs && (id < 0 || id != wid)) {
+      if (id >= 0) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) keep(r, my_id == id);
+      } else {
+        int row_id[16];
+        load_ids(row_id, walk.ids, qt + 4 * hi, N);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) keep(r, my_id == row_id[r]);
+      }
+    }
+    if constexpr (DO_DV) {
+      const F pf0 = acc_frag<T>(pm, 0), pf1 = acc_frag<T>(pm, 1);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        dv[db] = mma(rd.tr(ds, 0, db), pf0, dv[db]);
+        dv[db] = mma(rd.tr(ds, 16, db), pf1, dv[db]);
+      }
+    }
+    if constexpr (DO_DK) {
+      const F sf0 = acc_frag<T>(dsm, 0), sf1 = acc_frag<T>(dsm, 1);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        dk[db] = mma(rd.tr(qs, 0, db), sf0, dk[db]);
+        dk[db] = mma(rd.tr(qs, 16, db), sf1, dk[db]);
+      }
+    }
+  });
+
+  // ---- join the key block's waves: wave `sub` 0 takes the others' partials ----
+  if constexpr (SPLIT > 1) {
+    constexpr int REGS = 16 * DB;
+    static_assert((SPLIT - 1) * RW * REGS * 256 <= Ring::BYTES, "partials fit the ring");
+    auto join = [&](float16_t (&x)[DB]) {
+      __syncthreads();  // every wave is done reading the ring (or the previous partials)
+      if (sub > 0) {
+        lds_ptr<float> out = part_slot<REGS>(smem, wave - RW, lane);
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) out[(16 * db + r) * 64] = x[db][r];
+      }
+      __syncthreads();
+      if (sub == 0) {
+#pragma unroll
+        for (int w = 0; w < SPLIT - 1; ++w) {
+          lds_ptr<float> in = part_slot<REGS>(smem, w * RW + wave, lane);
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[db][r] += in[(16 * db + r) * 64];
+        }
+      }
+    };
+    if constexpr (DO_DV) join(dv);
+    if constexpr (DO_DK) join(dk);
+    if (sub > 0) return;
+  }
+
+  if (krow >= N) return;
+  T* dkp = static_cast<T*>(p.dk) + kbase + static_cast<size_t>(krow) * D;
+  T* dvp = static_cast<T*>(p.dv) + kbase + static_cast<size_t>(krow) * D;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int rr = 0; rr < 4; ++rr) {
+      const int d0 = 32 * db + 8 * rr + 4 * hi;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (ROWS == kRowFull || d0 + j < D) {
+          if constexpr (DO_DK) dkp[d0 + j] = static_cast<T>(dk[db][4 * rr + j] * p.scale);
+          if constexpr (DO_DV) dvp[d0 + j] = static_cast<T>(dv[db][4 * rr + j]);
+        }
+    }
+}
+
+}  // namespace scored
+}  // namespace fa

@@ -1,0 +1,91 @@
+// Launches of the scored-attention kernels, shared by the fp16 and the fp32
+// translation unit.
+#pragma once
+
+#include <algorithm>
+
+#include "capi_internal.h"
+#include "scored_kernels.h"
+
+namespace fa {
+namespace scored {
+
+// Deals `units` of `heads` heads over the XCDs (map_block).  Units that do not
+// fill the XCDs evenly leave some of them idle, so fewer than 32 that are no
+// multiple of eight are dealt block by block instead (group_units 0).
+inline long long deal(ScoredParams& p, long long units, int heads) {
+  p.units = static_cast<int>(units);
+  p.heads = heads;
+  if (units % kXcds != 0 && units < 4 * kXcds) {
+    p.group_units = 0;
+    return units * heads * p.nblk;
+  }
+  const long long per_xcd = (units + kXcds - 1) / kXcds;
+  const long long per_unit = static_cast<long long>(heads) * p.nblk;
+  constexpr long long kGroupWorkgroups = 128;  // an XCD's blocks in flight, about
+  p.group_units = static_cast<int>(std::max<long long>(1, std::min(per_xcd, (kGroupWorkgroups + per_unit - 1) / per_unit)));
+  return (per_xcd + p.group_units - 1) / p.group_units * p.group_units * kXcds * per_unit;
+}
+
+// A query-major grid: the heads of a KV head share a unit where the units then
+// still fill the XCDs.
+inline long long deal_query(ScoredParams& p) {
+  const long long units = static_cast<long long>(p.B) * p.H_KV;
+  if (units % kXcds == 0 || units >= 4 * kXcds) return deal(p, units, p.G);
+  return deal(p, static_cast<long long>(p.B) * p.H_Q, 1);
+}
+
+template <typename T, int DP, int DC, int ROWS, int MODE, int MODS>
+void launch_query(ScoredParams p, bool split, hipStream_t st) {
+  if (ROWS != kRowElems && split) {
+    p.nblk = ceil_div(p.N, kBlockRows / 2);
+    const dim3 grid(static_cast<unsigned>(deal_query(p)));
+    hipLaunchKernelGGL((scored_query_kernel<T, DP, DC, ROWS, MODE, ROWS == kRowElems ? 1 : 2, MODS>), grid, dim3(kThreads), 0, st, p);
+    return;
+  }
+  p.nblk = ceil_div(p.N, kBlockRows);
+  const dim3 grid(static_cast<unsigned>(deal_query(p)));
+  hipLaunchKernelGGL((scored_query_kernel<T, DP, DC, ROWS, MODE, 1, MODS>), grid, dim3(kThreads), 0, st, p);
+}
+
+template <typename T, int DP, int DC, int ROWS, int PASS, int MODS>
+void launch_key(ScoredParams p, bool split, hipStream_t st) {
+  const long long units = static_cast<long long>(p.B) * p.H_KV;
+  if (ROWS != kRowElems && split) {
+    p.nblk = ceil_div(p.N, kBlockRows / 2);
+    const dim3 grid(static_cast<unsigned>(deal(p, units, 1)));
+    hipLaunchKernelGGL((scored_key_kernel<T, DP, DC, ROWS, PASS, ROWS == kRowElems ? 1 : 2, MODS>), grid, dim3(kThreads), 0, st, p);
+    return;
+  }
+  p.nblk = ceil_div(p.N, kBlockRows);
+  const dim3 grid(static_cast<unsigned>(deal(p, units, 1)));
+  hipLaunchKernelGGL((scored_key_kernel<T, DP, DC, ROWS, PASS, 1, MODS>), grid, dim3(kThreads), 0, st, p);
+}
+
+// Split blocks (two waves a block, half the walk each) where 128-row blocks
+// would leave CUs idle or with little to switch to.
+constexpr long long kSplitMaxBlocks = 512;
+inline bool split_query(const ScoredParams& p) {
+  return static_cast<long long>(p.B) * p.H_Q * ceil_div(p.N, kBlockRows) <= kSplitMaxBlocks;
+}
+inline bool split_key(const ScoredParams& p) {
+  return static_cast<long long>(p.B) * p.H_KV * ceil_div(p.N, kBlockRows) <= kSplitMaxBlocks;
+}
+
+template <typename T, int DP, int DC, int ROWS, int MODS>
+void launch_backward_shape(const ScoredParams& p, hipStream_t st) {
+  launch_query<T, DP, DC, ROWS, 1, MODS>(p, split_query(p), st);
+  if constexpr (sizeof(T) == 2 && DP > 64) {
+    launch_key<T, DP, DC, ROWS, kPassDV, MODS>(p, split_key(p), st);
+    launch_key<T, DP, DC, ROWS, kPassDK, MODS>(p, split_key(p), st);
+  } else {
+    launch_key<T, DP, DC, ROWS, kPassBoth, MODS>(p, split_key(p), st);
+  }
+}
+
+// Entry points of the fp32 translation unit.
+void forward_fp32(const ScoredParams& p, bool vec, hipStream_t st);
+void backward_fp32(const ScoredParams& p, bool vec, hipStream_t st);
+
+}  // namespace scored
+}  // namespace fa

@@ -309,6 +309,51 @@ int fa_gather_heads(void* full, const void* local, int B, int total_heads,
 int fa_cross_gpu_allreduce_fp16(void* dst, const void* src, size_t n,
                                 void* stream);
 
+/*
+ * Self-attention with modified scores (no counterpart in the reference).
+ *   q/o [B, H_Q, N, D], k/v [B, H_KV, N, D], H_Q % H_KV == 0; fp16: D <= 256,
+ *   fp32: D <= 128.  lse fp32 [B, H_Q, N] or NULL (natural log).
+ *   s = q.k / sqrt(D); softcap != 0 (in [1e-3, 1e6]): s = softcap * tanh(s / softcap);
+ *   slopes fp32 [H_Q] or NULL: s -= slopes[h] * |i - j|.
+ *   Key j is visible to query i iff
+ *     doc_ids == NULL or doc_ids[b, i] == doc_ids[b, j] >= 0  (int32 [B, N]), and
+ *     not causal, or j <= i, or j < prefix_lens[b]  (int32 [B] or NULL; needs causal).
+ *   A row that sees no key (a negative id) has o = 0 and lse = -inf; what rows
+ *   of negative id hold, NaN included, reaches no other row.
+ */
+int fa_scored_fp16(const void* q, const void* k, const void* v, void* o,
+                   float* lse, int B, int H_Q, int H_KV, int N, int D,
+                   int causal, float softcap, const float* slopes,
+                   const int32_t* doc_ids, const int32_t* prefix_lens,
+                   void* stream);
+int fa_scored_fp32(const void* q, const void* k, const void* v, void* o,
+                   float* lse, int B, int H_Q, int H_KV, int N, int D,
+                   int causal, float softcap, const float* slopes,
+                   const int32_t* doc_ids, const int32_t* prefix_lens,
+                   void* stream);
+
+/*
+ * Its backward: dq [B, H_Q, N, D], dk/dv [B, H_KV, N, D] (summed over each KV
+ * head's query heads, in a fixed order, without atomics) from dout, the
+ * forward's inputs, its output and its lse.  D <= 128.  The workspace holds
+ * fa_backward_workspace_size(B, H_Q, N) bytes and needs no initialisation.
+ * softcap, slopes, doc_ids and prefix_lens are constants of the gradient.
+ */
+int fa_scored_backward_fp16(const void* dout, const void* q, const void* k,
+                            const void* v, const void* out, const float* lse,
+                            void* dq, void* dk, void* dv, int B, int H_Q,
+                            int H_KV, int N, int D, int causal, float softcap,
+                            const float* slopes, const int32_t* doc_ids,
+                            const int32_t* prefix_lens, void* workspace,
+                            size_t workspace_bytes, void* stream);
+int fa_scored_backward_fp32(const void* dout, const void* q, const void* k,
+                            const void* v, const void* out, const float* lse,
+                            void* dq, void* dk, void* dv, int B, int H_Q,
+                            int H_KV, int N, int D, int causal, float softcap,
+                            const float* slopes, const int32_t* doc_ids,
+                            const int32_t* prefix_lens, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

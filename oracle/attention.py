@@ -552,3 +552,54 @@ def allreduce_fp16(dst, src):
     with np.errstate(over="ignore", invalid="ignore"):
         s = (a + b).astype(np.float32).astype(np.float16)
     return torch.from_numpy(s).reshape(dst.shape)
+
+
+def scored_visible(n, causal, doc_ids=None, prefix_lens=None, b=0):
+    """[n, n] mask of what attention with modified scores lets query i see of key j in batch row b."""
+    i = torch.arange(n)
+    see = torch.ones(n, n, dtype=torch.bool)
+    if causal:
+        see = i[None, :] <= i[:, None]
+        if prefix_lens is not None:
+            see = see | (i[None, :] < int(prefix_lens[b]))
+    if doc_ids is not None:
+        ids = doc_ids[b]
+        see = see & (ids[None, :] == ids[:, None]) & (ids >= 0)[None, :]
+    return see
+
+
+def scored(q, k, v, causal, softcap=0.0, slopes=None, doc_ids=None, prefix_lens=None):
+    """Attention with capped, biased and masked scores in 64 bits: (out, lse, P, scores before the mask).
+
+    s = q.k / sqrt(D); c = softcap tanh(s / softcap); y = c - slope |i - j|; softmax over the
+    visible keys.  A row that sees none has out 0 and lse -inf; rows of negative id are taken as
+    zeros, whatever they hold."""
+    b_, h_q, n, d = q.shape
+    q, k, v = (t.double() for t in (q, k, v))
+    if doc_ids is not None:
+        pad = (doc_ids < 0)[:, None, :, None]
+        q, k, v = (torch.where(pad, torch.zeros_like(t), t) for t in (q, k, v))
+    k, v = expand_kv(k, h_q), expand_kv(v, h_q)
+    y = torch.matmul(q, k.transpose(-1, -2)) / math.sqrt(d)
+    if softcap:
+        y = softcap * torch.tanh(y / softcap)
+    if slopes is not None:
+        i = torch.arange(n).double()
+        y = y - slopes.double()[:, None, None] * (i[:, None] - i[None, :]).abs()
+    see = torch.stack([scored_visible(n, causal, doc_ids, prefix_lens, b) for b in range(b_)])[:, None]
+    top = torch.where(see, y, torch.full_like(y, -1e300)).amax(-1, keepdim=True).detach()
+    w = torch.exp(torch.where(see, y - top, torch.full_like(y, -math.inf)))
+    total = w.sum(-1, keepdim=True)
+    p = w / torch.where(total > 0, total, torch.ones_like(total))
+    lse = torch.where(total > 0, top + torch.log(total), torch.full_like(total, -math.inf))[..., 0]
+    return torch.matmul(p, v), lse, p, y
+
+
+def scored_backward(dout, q, k, v, causal, softcap=0.0, slopes=None, doc_ids=None, prefix_lens=None):
+    """(dq, dk, dv) of ``scored`` in 64 bits, by automatic differentiation of its definition."""
+    q, k, v = (t.detach().double().requires_grad_() for t in (q, k, v))
+    out = scored(q, k, v, causal, softcap, slopes, doc_ids, prefix_lens)[0]
+    do = dout.double()
+    if doc_ids is not None:
+        do = torch.where((doc_ids < 0)[:, None, :, None], torch.zeros_like(do), do)
+    return torch.autograd.grad(out, (q, k, v), do)
