@@ -45,7 +45,8 @@ HOT_PATH = (
 
 # Operators this build adds beside the reference's.
 ADDED_NAMES = (
-    "forward_scored", "forward_scored_with_lse", "backward_scored",
+    "forward_scored", "forward_scored_with_lse", "backward_scored", "forward_decode_scored_gqa_fp16",
+    "append_paged_kv8", "forward_paged_decode_kv8_gqa", "forward_decode_weighted_gqa_fp16", "evict_by_weight",
 )
 
 for _name in API_NAMES + ADDED_NAMES:

@@ -762,6 +762,190 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> backward_scored(at::Tensor dout, 
   return std::make_tuple(dq, dk, dv);
 }
 
+// ---------------------------------------------------------------------------
+// Single-token attention with modified scores, and the caches around it (no
+// counterparts in the reference).
+
+// Checks of a ragged contiguous cache: cache_lens int32 [B], as continuous batching.
+void check_ragged_cache(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cache_lens) {
+  CHECK_INPUT(q);
+  CHECK_INPUT(k);
+  CHECK_INPUT(v);
+  CHECK_INPUT(cache_lens);
+  check_decode_gqa_input_shapes(q, k, v);
+  TORCH_CHECK(q.dtype() == at::kHalf, "q, k, v must be float16");
+  TORCH_CHECK(q.size(2) == 1, "q sequence length must be 1 for decode mode");
+  TORCH_CHECK(k.size(1) > 0 && q.size(1) >= k.size(1), "H_Q must be >= H_KV");
+  TORCH_CHECK(q.size(1) % k.size(1) == 0, "H_Q must be divisible by H_KV");
+  TORCH_CHECK(q.size(3) <= kMaxDLarge, "D must be <= MAX_D_LARGE(256)");
+  TORCH_CHECK(cache_lens.dtype() == at::kInt, "cache_lens must be int32");
+  TORCH_CHECK(cache_lens.dim() == 1 && cache_lens.size(0) == q.size(0), "cache_lens must be [B]");
+  CHECK_SAME_DEVICE(q, cache_lens);
+}
+
+at::Tensor forward_decode_scored_gqa_fp16(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cache_lens, double softcap,
+                                          OptTensor slopes) {
+  check_ragged_cache(q, k, v, cache_lens);
+  check_softcap(softcap);
+  const float* sl = optional_ptr<float>(slopes, q, "slopes", at::kFloat, {q.size(1)});
+  HIPGuardMasqueradingAsCUDA guard(q.device());
+  const int B = to_int(q.size(0), "B"), hq = to_int(q.size(1), "H_Q"), hkv = to_int(k.size(1), "H_KV");
+  const int n = to_int(k.size(2), "N"), d = to_int(q.size(3), "D");
+  auto out = at::empty_like(q);
+  auto ws = decode_workspace(q, B, hq, hkv, n, d);
+  check_fa(fa_decode_scored_fp16(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cache_lens.data_ptr<int32_t>(), B,
+                                 hq, hkv, n, d, static_cast<float>(softcap), sl, ws_ptr(ws), ws_bytes(ws), cur_stream()));
+  return out;
+}
+
+// weight [B, H_KV, N] float32; the sums go to weight_out (default: weight itself).
+std::tuple<at::Tensor, at::Tensor> forward_decode_weighted_gqa_fp16(at::Tensor q, at::Tensor k, at::Tensor v,
+                                                                    at::Tensor cache_lens, at::Tensor weight,
+                                                                    OptTensor weight_out, double softcap,
+                                                                    OptTensor slopes) {
+  check_ragged_cache(q, k, v, cache_lens);
+  check_softcap(softcap);
+  const at::IntArrayRef sizes = k.sizes().slice(0, 3);
+  const float* w = optional_ptr<float>(weight, q, "weight", at::kFloat, sizes);
+  const float* wo = optional_ptr<float>(weight_out, q, "weight_out", at::kFloat, sizes);
+  const float* sl = optional_ptr<float>(slopes, q, "slopes", at::kFloat, {q.size(1)});
+  HIPGuardMasqueradingAsCUDA guard(q.device());
+  const int B = to_int(q.size(0), "B"), hq = to_int(q.size(1), "H_Q"), hkv = to_int(k.size(1), "H_KV");
+  const int n = to_int(k.size(2), "N"), d = to_int(q.size(3), "D");
+  auto out = at::empty_like(q);
+  auto ws = decode_workspace(q, B, hq, hkv, n, d);
+  const size_t bytes = fa_decode_weighted_scratch_size(B, hq, n);
+  auto scratch = at::empty({static_cast<int64_t>(bytes / sizeof(float))}, q.options().dtype(at::kFloat));
+  check_fa(fa_decode_weighted_fp16(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cache_lens.data_ptr<int32_t>(),
+                                   w, const_cast<float*>(wo ? wo : w), B, hq, hkv, n, d, static_cast<float>(softcap), sl,
+                                   scratch.data_ptr(), bytes, ws_ptr(ws), ws_bytes(ws), cur_stream()));
+  return std::make_tuple(out, weight_out.has_value() ? *weight_out : weight);
+}
+
+// Checks of an 8-bit paged cache: codes [pages, H_KV, page, D] int8 or e4m3, scales
+// [pages, H_KV] float32, block_table int32 [B, max_blocks].  Returns whether it holds e4m3.
+bool check_kv8(const at::Tensor& like, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& k_scale,
+               const at::Tensor& v_scale, const at::Tensor& block_table, int64_t B, int64_t D) {
+  CHECK_INPUT(k_cache);
+  CHECK_INPUT(v_cache);
+  CHECK_INPUT(k_scale);
+  CHECK_INPUT(v_scale);
+  CHECK_INPUT(block_table);
+  CHECK_DIM(k_cache, 4);
+  CHECK_DIM(block_table, 2);
+  for (const at::Tensor* t : {&k_cache, &v_cache, &k_scale, &v_scale, &block_table})
+    TORCH_CHECK(t->device() == like.device(), "all tensors must be on the same device");
+  TORCH_CHECK(k_cache.scalar_type() == at::kChar || k_cache.scalar_type() == at::kFloat8_e4m3fn,
+              "k_cache must be int8 or float8_e4m3fn");
+  CHECK_SAME_DTYPE(k_cache, v_cache);
+  TORCH_CHECK(k_cache.sizes() == v_cache.sizes(), "k_cache and v_cache must have the same shape");
+  TORCH_CHECK(k_cache.size(3) == D, "k_cache head dimension must match");
+  const auto page = k_cache.size(2);
+  TORCH_CHECK(page == 16 || page == 32 || page == 64 || page == 128 || page == 256,
+              "the cache's page must be 16, 32, 64, 128 or 256 tokens");
+  TORCH_CHECK(k_scale.dtype() == at::kFloat && v_scale.dtype() == at::kFloat, "k_scale and v_scale must be float32");
+  TORCH_CHECK(k_scale.sizes() == k_cache.sizes().slice(0, 2) && v_scale.sizes() == k_scale.sizes(),
+              "k_scale and v_scale must be [num_pages, H_KV]");
+  TORCH_CHECK(block_table.dtype() == at::kInt, "block_table must be int32");
+  TORCH_CHECK(block_table.size(0) == B, "block_table batch size must match");
+  TORCH_CHECK(D <= kMaxDLarge, "D must be <= MAX_D_LARGE(256)");
+  return k_cache.scalar_type() == at::kFloat8_e4m3fn;
+}
+
+// k, v [total, H_KV, D] float16: sequence b's new tokens are rows [cu_seqlens[b], cu_seqlens[b + 1])
+// and go to its positions cache_lens[b] ..; in place.
+void append_paged_kv8(at::Tensor k, at::Tensor v, at::Tensor cu_seqlens, at::Tensor cache_lens, int64_t max_new,
+                      at::Tensor k_cache, at::Tensor v_cache, at::Tensor k_scale, at::Tensor v_scale,
+                      at::Tensor block_table) {
+  CHECK_INPUT(k);
+  CHECK_INPUT(v);
+  CHECK_INPUT(cu_seqlens);
+  CHECK_INPUT(cache_lens);
+  CHECK_DIM(k, 3);
+  TORCH_CHECK(k.sizes() == v.sizes(), "k and v must have the same shape");
+  TORCH_CHECK(k.dtype() == at::kHalf && v.dtype() == at::kHalf, "k and v must be float16");
+  CHECK_SAME_DEVICE(k, v);
+  CHECK_SAME_DEVICE(k, cu_seqlens);
+  CHECK_SAME_DEVICE(k, cache_lens);
+  TORCH_CHECK(cu_seqlens.dtype() == at::kInt && cache_lens.dtype() == at::kInt, "cu_seqlens and cache_lens must be int32");
+  CHECK_DIM(cache_lens, 1);
+  TORCH_CHECK(cu_seqlens.dim() == 1 && cu_seqlens.size(0) == cache_lens.size(0) + 1, "cu_seqlens must be [B + 1]");
+  TORCH_CHECK(max_new > 0, "max_new must be positive");
+  const bool fp8 = check_kv8(k, k_cache, v_cache, k_scale, v_scale, block_table, cache_lens.size(0), k.size(2));
+  TORCH_CHECK(k_cache.size(1) == k.size(1), "k_cache head count must match k");
+  TORCH_CHECK(k.size(1) > 0, "k must have a head");
+  HIPGuardMasqueradingAsCUDA guard(k.device());
+  check_fa(fa_paged_append_kv8(k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr<int32_t>(), cache_lens.data_ptr<int32_t>(),
+                               k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr<float>(), v_scale.data_ptr<float>(),
+                               block_table.data_ptr<int32_t>(), fp8 ? 1 : 0, to_int(cache_lens.size(0), "B"),
+                               to_int(k.size(0), "total"), to_int(std::min<int64_t>(max_new, INT32_MAX), "max_new"),
+                               to_int(k.size(1), "H_KV"), to_int(k.size(2), "D"), to_int(k_cache.size(0), "num_pages"),
+                               to_int(k_cache.size(2), "page"), to_int(block_table.size(1), "max_blocks"), cur_stream()));
+}
+
+at::Tensor forward_paged_decode_kv8_gqa(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at::Tensor k_scale,
+                                        at::Tensor v_scale, at::Tensor block_table, at::Tensor seq_lens, double softcap,
+                                        OptTensor slopes) {
+  CHECK_INPUT(q);
+  CHECK_INPUT(seq_lens);
+  CHECK_DIM(q, 4);
+  CHECK_SAME_DEVICE(q, seq_lens);
+  TORCH_CHECK(q.dtype() == at::kHalf, "q must be float16");
+  TORCH_CHECK(q.size(2) == 1, "q sequence length must be 1 for decode mode");
+  TORCH_CHECK(seq_lens.dtype() == at::kInt, "seq_lens must be int32");
+  TORCH_CHECK(seq_lens.dim() == 1 && seq_lens.size(0) == q.size(0), "seq_lens must be [B]");
+  const bool fp8 = check_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, q.size(0), q.size(3));
+  TORCH_CHECK(k_cache.size(1) > 0 && q.size(1) >= k_cache.size(1), "H_Q must be >= H_KV");
+  TORCH_CHECK(q.size(1) % k_cache.size(1) == 0, "H_Q must be divisible by H_KV");
+  check_softcap(softcap);
+  const float* sl = optional_ptr<float>(slopes, q, "slopes", at::kFloat, {q.size(1)});
+  HIPGuardMasqueradingAsCUDA guard(q.device());
+  const int B = to_int(q.size(0), "B"), hq = to_int(q.size(1), "H_Q"), hkv = to_int(k_cache.size(1), "H_KV");
+  const int d = to_int(q.size(3), "D"), page = to_int(k_cache.size(2), "page"), blocks = to_int(block_table.size(1), "max_blocks");
+  auto out = at::empty_like(q);
+  auto ws = decode_workspace(q, B, hq, hkv, to_int(static_cast<int64_t>(blocks) * page, "table row tokens"), d);
+  check_fa(fa_paged_decode_kv8(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr<float>(),
+                               v_scale.data_ptr<float>(), out.data_ptr(), block_table.data_ptr<int32_t>(),
+                               seq_lens.data_ptr<int32_t>(), fp8 ? 1 : 0, B, hq, hkv, d, to_int(k_cache.size(0), "num_pages"),
+                               page, blocks, static_cast<float>(softcap), sl, ws_ptr(ws), ws_bytes(ws), cur_stream()));
+  return out;
+}
+
+// (k_out, v_out [B, H_KV, capacity, D], weight_out, index [B, H_KV, capacity], new_lens [B])
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> evict_by_weight(
+    at::Tensor k, at::Tensor v, at::Tensor weight, at::Tensor seq_lens, int64_t budget, int64_t recent, int64_t capacity) {
+  CHECK_INPUT(k);
+  CHECK_INPUT(v);
+  CHECK_INPUT(weight);
+  CHECK_INPUT(seq_lens);
+  CHECK_DIM(k, 4);
+  TORCH_CHECK(k.dtype() == at::kHalf && v.dtype() == at::kHalf, "k and v must be float16");
+  TORCH_CHECK(k.sizes() == v.sizes(), "k and v must have the same shape");
+  CHECK_SAME_DEVICE(k, v);
+  CHECK_SAME_DEVICE(k, weight);
+  CHECK_SAME_DEVICE(k, seq_lens);
+  TORCH_CHECK(weight.dtype() == at::kFloat, "weight must be float32");
+  TORCH_CHECK(weight.sizes() == k.sizes().slice(0, 3), "weight must be [B, H_KV, N]");
+  TORCH_CHECK(seq_lens.dtype() == at::kInt, "seq_lens must be int32");
+  TORCH_CHECK(seq_lens.dim() == 1 && seq_lens.size(0) == k.size(0), "seq_lens must be [B]");
+  TORCH_CHECK(recent >= 0 && recent <= budget, "recent must lie in [0, budget]");
+  TORCH_CHECK(budget <= capacity, "budget must not exceed capacity");
+  TORCH_CHECK(k.size(1) > 0 && k.size(3) > 0, "k must have a head and a head dimension");
+  const int B = to_int(k.size(0), "B"), h = to_int(k.size(1), "H_KV"), n = to_int(k.size(2), "N"), d = to_int(k.size(3), "D");
+  const int cap = to_int(capacity, "capacity");
+  HIPGuardMasqueradingAsCUDA guard(k.device());
+  auto k_out = at::empty({k.size(0), k.size(1), capacity, k.size(3)}, k.options());
+  auto v_out = at::empty_like(k_out);
+  auto weight_out = at::empty({k.size(0), k.size(1), capacity}, weight.options());
+  auto index = at::empty({k.size(0), k.size(1), capacity}, seq_lens.options());
+  auto new_lens = at::empty({k.size(0)}, seq_lens.options());
+  check_fa(fa_evict_by_weight(k.data_ptr(), v.data_ptr(), weight.data_ptr<float>(), seq_lens.data_ptr<int32_t>(),
+                              k_out.data_ptr(), v_out.data_ptr(), weight_out.data_ptr<float>(), index.data_ptr<int32_t>(),
+                              new_lens.data_ptr<int32_t>(), B, h, n, d, static_cast<int>(budget), static_cast<int>(recent), cap,
+                              cur_stream()));
+  return std::make_tuple(k_out, v_out, weight_out, index, new_lens);
+}
+
 // token_eviction (flash_attn_kernel.cu:4296-4344): (k_out, v_out, valid_mask).
 std::tuple<at::Tensor, at::Tensor, at::Tensor> token_eviction(at::Tensor k, at::Tensor v, at::Tensor attn_scores,
                                                               int num_evict) {
@@ -1084,5 +1268,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("q"), py::arg("k"), py::arg("v"), py::arg("out"), py::arg("logsumexp"), py::arg("causal"),
         py::arg("softcap") = 0.0, py::arg("slopes") = py::none(), py::arg("doc_ids") = py::none(),
         py::arg("prefix_lens") = py::none());
+  m.def("forward_decode_scored_gqa_fp16", &forward_decode_scored_gqa_fp16,
+        "GQA decode with capped or biased scores over a ragged cache (MI355X split-KV)", py::arg("q"), py::arg("k"),
+        py::arg("v"), py::arg("cache_lens"), py::arg("softcap") = 0.0, py::arg("slopes") = py::none());
+  m.def("forward_decode_weighted_gqa_fp16", &forward_decode_weighted_gqa_fp16,
+        "GQA decode that adds up each cached token's attention weight (MI355X split-KV)", py::arg("q"), py::arg("k"),
+        py::arg("v"), py::arg("cache_lens"), py::arg("weight"), py::arg("weight_out") = py::none(),
+        py::arg("softcap") = 0.0, py::arg("slopes") = py::none());
+  m.def("append_paged_kv8", &append_paged_kv8, "Append tokens to an 8-bit paged KV cache (MI355X)", py::arg("k"),
+        py::arg("v"), py::arg("cu_seqlens"), py::arg("cache_lens"), py::arg("max_new"), py::arg("k_cache"),
+        py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("block_table"));
+  m.def("forward_paged_decode_kv8_gqa", &forward_paged_decode_kv8_gqa,
+        "Paged GQA decode over an 8-bit cache with page scales (MI355X split-KV)", py::arg("q"), py::arg("k_cache"),
+        py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("block_table"), py::arg("seq_lens"),
+        py::arg("softcap") = 0.0, py::arg("slopes") = py::none());
+  m.def("evict_by_weight", &evict_by_weight, "KV-cache eviction by accumulated attention weight (MI355X)", py::arg("k"),
+        py::arg("v"), py::arg("weight"), py::arg("seq_lens"), py::arg("budget"), py::arg("recent"), py::arg("capacity"));
   m.def("_fa_version", []() { return std::string(fa_version()); });
 }

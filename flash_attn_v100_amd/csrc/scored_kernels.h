@@ -207,12 +207,6 @@ struct TileWalk {
 };
 
 // ---- scores ----
-// tanh z = z (1 + w P(w)), w = z^2, for |z| <= 1/2: P fitted to the least
-// largest relative error (1.5e-8; 7.4e-8 evaluated in fp32).
-constexpr float kTanhMax = 0.5f;
-constexpr float kT0 = -0.333331435918808f, kT1 = 0.13325878977775574f, kT2 = -0.05304547771811485f,
-                kT3 = 0.01724146120250225f;
-
 // Raw products s -> capped scores in the log2 domain, cap log2(e) tanh(s scale / cap).
 // Where every |z| of the wave's tile is at most 1/2 (scores below half the
 // cap) the polynomial serves: 8 full-rate operations a score where the
@@ -229,17 +223,13 @@ __device__ __forceinline__ void cap_scores(float16_t& s, const ScoredParams& p) 
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     const float w = z[r] * z[r];
-    const float pw = fmaf(fmaf(fmaf(kT3, w, kT2), w, kT1), w, kT0);
     const float zc = z[r] * p.cap_log2;
-    s[r] = fmaf(zc * w, pw, zc);
+    s[r] = fmaf(zc * w, tanh_p(w), zc);
   }
   if (far) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      // 1 - 2 / (e^2|z| + 1): at least 0.46 here, so nothing cancels
-      const float e = fast_exp2(fabsf(z[r]) * (2.0f * kLog2e));
-      const float t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
-      const float y = __builtin_copysignf(t * p.cap_log2, z[r]);
+      const float y = __builtin_copysignf(tanh_far(z[r]) * p.cap_log2, z[r]);
       s[r] = fabsf(z[r]) <= kTanhMax ? s[r] : y;
       // (NaN compares false and comes through the exponential)
     }

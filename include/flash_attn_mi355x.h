@@ -354,6 +354,93 @@ int fa_scored_backward_fp32(const void* dout, const void* q, const void* k,
                             const int32_t* prefix_lens, void* workspace,
                             size_t workspace_bytes, void* stream);
 
+/*
+ * Single-token form of fa_scored_*, over a contiguous cache of per-sequence
+ * lengths (as fa_continuous_batching_fp16): q/o [B, H_Q, 1, D], k/v [B, H_KV, N,
+ * D] fp16, D <= 256; sequence b attends keys [0, min(cache_lens[b] + 1, N)), the
+ * query being the last of them.  softcap and slopes as above.  A sequence that
+ * attends nothing has o = 0.  Workspace as for fa_decode_fp16 (max_len = N).
+ */
+int fa_decode_scored_fp16(const void* q, const void* k, const void* v, void* o,
+                          const int32_t* cache_lens, int B, int H_Q, int H_KV,
+                          int N, int D, float softcap, const float* slopes,
+                          void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/*
+ * fa_decode_scored_fp16 that also adds up what each key was attended with:
+ *   weight_out[b, h_kv, t] = weight[b, h_kv, t] + sum over the KV head's query
+ *   heads of their softmax weight of key t, for the keys attended; other
+ *   entries of weight_out are left as they are.  weight/weight_out fp32 [B,
+ *   H_KV, N]; they may be one array.  The scratch holds
+ *   fa_decode_weighted_scratch_size(B, H_Q, N) bytes and needs no initialisation.
+ *   B * H_KV <= 65535.  Two launches.
+ */
+size_t fa_decode_weighted_scratch_size(int B, int H_Q, int N);
+int fa_decode_weighted_fp16(const void* q, const void* k, const void* v,
+                            void* o, const int32_t* cache_lens,
+                            const float* weight, float* weight_out, int B,
+                            int H_Q, int H_KV, int N, int D, float softcap,
+                            const float* slopes, void* scratch,
+                            size_t scratch_bytes, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/*
+ * Append to a paged cache held in 8 bits with a scale for each page and head.
+ *   k/v fp16 [total, H_KV, D], D <= 256: sequence b's new tokens are rows
+ *   [cu_seqlens[b], cu_seqlens[b + 1]), its first max_new of them, and go to its
+ *   positions cache_lens[b], cache_lens[b] + 1, ...  Position t lives in page
+ *   block_table[b, t / page] (int32 [B, max_blocks]), row t % page.
+ *   k_cache/v_cache [num_pages, H_KV, page, D]: int8 codes, or e4m3 with fp8;
+ *   k_scale/v_scale fp32 [num_pages, H_KV]; page 16, 32, 64, 128 or 256.
+ *   A value is code * scale; scale = max |x| / 127 (e4m3: 448) over the page's
+ *   tokens of the head, code = x / scale rounded to nearest even.  In a page
+ *   that already holds tokens of the sequence the scale only grows, and where it
+ *   does the old codes are rounded again.  Rows of a page that are neither new
+ *   nor before the new ones are left as they are.  Tokens past the table row or
+ *   in a page outside [0, num_pages) are dropped.  Pages that receive tokens must
+ *   belong to one sequence each; inputs must be finite.  One launch.
+ */
+int fa_paged_append_kv8(const void* k, const void* v,
+                        const int32_t* cu_seqlens, const int32_t* cache_lens,
+                        void* k_cache, void* v_cache, float* k_scale,
+                        float* v_scale, const int32_t* block_table, int fp8,
+                        int B, int total, int max_new, int H_KV, int D,
+                        int num_pages, int page, int max_blocks, void* stream);
+
+/*
+ * Paged GQA decode over that cache: q/o fp16 [B, H_Q, 1, D]; sequence b attends
+ * tokens [0, seq_lens[b]).  softcap and slopes as for fa_decode_scored_fp16.  An
+ * empty sequence has o = 0; a page id outside [0, num_pages) or a length past the
+ * table row (page * max_blocks) gives NaN for that sequence.  Workspace as for
+ * fa_decode_fp16 (max_len = page * max_blocks).
+ */
+int fa_paged_decode_kv8(const void* q, const void* k_cache,
+                        const void* v_cache, const float* k_scale,
+                        const float* v_scale, void* o,
+                        const int32_t* block_table, const int32_t* seq_lens,
+                        int fp8, int B, int H_Q, int H_KV, int D,
+                        int num_pages, int page, int max_blocks, float softcap,
+                        const float* slopes, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/*
+ * KV-cache eviction by accumulated weight, per (sequence, KV head).
+ *   k/v fp16 [B, H_KV, N, D], weight fp32 [B, H_KV, N], seq_lens int32 [B]
+ *   (tokens held, at most N).  Of L > budget tokens the last `recent` stay and, of
+ *   the others, the budget - recent of greatest weight (ties: lower index first;
+ *   NaN counts as lightest); of L <= budget tokens all.  The kept rows are written
+ *   in their order to the front of k_out/v_out [B, H_KV, capacity, D], their weights
+ *   to weight_out and their old positions to index (int32) [B, H_KV, capacity];
+ *   rows past them are 0, 0 and -1.  new_lens[b] = min(L, budget).
+ *   0 <= recent <= budget <= capacity; B * H_KV <= 65535.  Two launches.
+ */
+int fa_evict_by_weight(const void* k, const void* v, const float* weight,
+                       const int32_t* seq_lens, void* k_out, void* v_out,
+                       float* weight_out, int32_t* index, int32_t* new_lens,
+                       int B, int H_KV, int N, int D, int budget, int recent,
+                       int capacity, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

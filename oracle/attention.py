@@ -603,3 +603,101 @@ def scored_backward(dout, q, k, v, causal, softcap=0.0, slopes=None, doc_ids=Non
     if doc_ids is not None:
         do = torch.where((doc_ids < 0)[:, None, :, None], torch.zeros_like(do), do)
     return torch.autograd.grad(out, (q, k, v), do)
+
+
+def scored_decode(q, k, v, lens, softcap=0.0, slopes=None):
+    """Single-token attention in 64 bits over the first lens[b] rows of k, v [B, H_KV, N, D]:
+    (out [B, H_Q, 1, D], P [B, H_Q, N], scores [B, H_Q, N]); a sequence of no rows gives zeros."""
+    b_, h_q, _, d = q.shape
+    n = k.shape[2]
+    out = torch.zeros(b_, h_q, 1, d, dtype=torch.float64)
+    p, y = torch.zeros(b_, h_q, n, dtype=torch.float64), torch.zeros(b_, h_q, n, dtype=torch.float64)
+    for b in range(b_):
+        m = max(0, min(int(lens[b]), n))
+        if m == 0:
+            continue
+        kb, vb = (expand_kv(t[b:b + 1, :, :m].double(), h_q)[0] for t in (k, v))
+        s = torch.matmul(kb, q[b, :, 0].double()[:, :, None])[..., 0] / math.sqrt(d)
+        if softcap:
+            s = softcap * torch.tanh(s / softcap)
+        if slopes is not None:
+            s = s - slopes.double()[:, None] * torch.arange(m - 1, -1, -1).double()
+        w = torch.softmax(s, -1)
+        y[b, :, :m], p[b, :, :m] = s, w
+        out[b, :, 0] = torch.matmul(w[:, None], vb)[:, 0]
+    return out, p, y
+
+
+KV8_TOP = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+
+
+def kv8_codes(x, scale, dtype):
+    """x fp32 as codes of scale: the fp32 quotient, clamped and rounded to nearest even (0 for scale 0)."""
+    top = KV8_TOP[dtype]
+    y = torch.where(scale > 0, x / scale, torch.zeros_like(x)).clamp(-top, top)
+    return y.round().to(dtype) if dtype == torch.int8 else y.to(dtype)
+
+
+def append_paged_kv8(k, v, cu, lens, max_new, k_cache, v_cache, k_scale, v_scale, table):
+    """The 8-bit paged append on copies: (k_cache, v_cache, k_scale, v_scale)."""
+    got = []
+    pages, h, page, _ = k_cache.shape
+    for new, cache, scales in ((k, k_cache, k_scale), (v, v_cache, v_scale)):
+        dtype, cache, scales = cache.dtype, cache.clone(), scales.clone()
+        for b in range(len(lens)):
+            lo, hi = max(0, min(int(cu[b]), new.shape[0])), max(0, min(int(cu[b + 1]), new.shape[0]))
+            at, end = int(lens[b]), int(lens[b]) + min(hi - lo, max_new)
+            while 0 <= at < end:
+                upto = min(end, (at // page + 1) * page)
+                pg = int(table[b, at // page]) if at // page < table.shape[1] else -1
+                if 0 <= pg < pages:
+                    x = new[lo + at - int(lens[b]):lo + upto - int(lens[b])].float().transpose(0, 1)
+                    scale = x.abs().amax((1, 2)) / torch.tensor(KV8_TOP[dtype])
+                    first = at % page
+                    if first:
+                        before = scales[pg]
+                        scale = torch.maximum(scale, before)
+                        again = kv8_codes(cache[pg, :, :first].float() * before[:, None, None], scale[:, None, None], dtype)
+                        keep = torch.where((scale > before)[:, None, None], again.float(), cache[pg, :, :first].float())
+                        cache[pg, :, :first] = keep.to(dtype)
+                    cache[pg, :, first:first + upto - at] = kv8_codes(x, scale[:, None, None], dtype)
+                    scales[pg] = scale
+                at = upto
+        got += [cache, scales]
+    return got[0], got[2], got[1], got[3]
+
+
+def paged_kv8_rows(cache, scale, table, lens):
+    """The values an 8-bit paged cache stands for, [B, H_KV, max(lens), D] in 64 bits, zeros past each length."""
+    _, h, page, d = cache.shape
+    n = max(1, max(int(x) for x in lens))
+    out = torch.zeros(len(lens), h, n, d, dtype=torch.float64)
+    for b, m in enumerate(int(x) for x in lens):
+        for t0 in range(0, m, page):
+            pg, t1 = int(table[b, t0 // page]), min(m, t0 + page)
+            out[b, :, t0:t1] = cache[pg, :, :t1 - t0].float().double() * scale[pg].double()[:, None, None]
+    return out
+
+
+def evict_by_weight(k, v, weight, lens, budget, recent, capacity):
+    """(k_out, v_out, weight_out, index, new_lens) of the eviction by weight, token by token."""
+    b_, h_, n, d = k.shape
+    k_out, v_out = (torch.zeros(b_, h_, capacity, d, dtype=k.dtype) for _ in range(2))
+    w_out, index = torch.zeros(b_, h_, capacity), torch.full((b_, h_, capacity), -1, dtype=torch.int32)
+    new_lens = torch.zeros(b_, dtype=torch.int32)
+    for b in range(b_):
+        m = max(0, min(int(lens[b]), n))
+        new_lens[b] = min(m, budget)
+        for h in range(h_):
+            rows = list(range(m))
+            if m > budget:
+                head = m - recent
+                key = lambda t: (-math.inf if math.isnan(x := float(weight[b, h, t])) else x)
+                nan = lambda t: math.isnan(float(weight[b, h, t]))
+                order = sorted(range(head), key=lambda t: (nan(t), -key(t), t))
+                rows = sorted(order[:budget - recent]) + list(range(head, m))
+            for r, t in enumerate(rows):
+                index[b, h, r] = t
+                w_out[b, h, r] = weight[b, h, t]
+                k_out[b, h, r], v_out[b, h, r] = k[b, h, t], v[b, h, t]
+    return k_out, v_out, w_out, index, new_lens
