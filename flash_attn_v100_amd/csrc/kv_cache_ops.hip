@@ -3,11 +3,12 @@
 //
 // ---- append (fa_paged_append_kv8) ----
 // A page of one head has one scale for its keys and one for its values:
-//   scale = max |x| / top over the page's tokens (top: 127 int8, 448 e4m3)
+//   scale = max |x| (1 / top) over the page's tokens (top: 127 int8, 448 e4m3)
 //   code  = x / scale, clamped to +-top and rounded to nearest even
 // A page that already holds tokens keeps the larger of its scale and the new
 // tokens' one; where it grows, the old codes are rounded again, code * old /
-// new.  Quotients are IEEE fp32 divisions, so codes are reproducible.
+// new.  All of it is IEEE fp32 arithmetic as written (1 / top rounded, one
+// product; the quotients correctly rounded), so codes are reproducible.
 // One wave per (page, head, K or V) does all of it: it alone reads and writes
 // that page's codes and scale, so no barrier and no atomics.  Bound by bytes
 // (2 read and 1 written a value): up to four 16-value chunks a lane stay in
@@ -101,7 +102,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
   const int id = p.block_table[b * p.max_blocks + pi];
   if (id < 0 || id >= p.num_pages) return;
 
-  constexpr float kTop = FP8 ? 448.0f : 127.0f;
+  constexpr float kTop = FP8 ? 448.0f : 127.0f, kInvTop = 1.0f / kTop;
   const int D = p.D;
   const int first = static_cast<int>(start & (page - 1));  // rows [first, first + rows) of the page are new
   const int rows = static_cast<int>(end - start);
@@ -141,7 +142,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
       raise(x);
     }
     const float amax = wave_max(fmaxf(static_cast<float>(top2[0]), static_cast<float>(top2[1])));
-    const float scale = fmaxf(amax / kTop, before);
+    const float scale = fmaxf(amax * kInvTop, before);
     auto store = [&](int c, const u32x4 (&x)[2]) {
       u32x4 codes;
 #pragma unroll
@@ -185,7 +186,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
     float amax = 0.0f;
     for (int e = lane; e < values; e += 64) amax = fmaxf(amax, fabsf(static_cast<float>(src[static_cast<size_t>(e / D) * stride + e % D])));
     amax = wave_max(amax);
-    const float scale = fmaxf(amax / kTop, before);
+    const float scale = fmaxf(amax * kInvTop, before);
     for (int e = lane; e < values; e += 64) {
       const float y = quotient(static_cast<float>(src[static_cast<size_t>(e / D) * stride + e % D]), scale, kTop);
       dst[static_cast<size_t>(first) * D + e] = static_cast<uint8_t>(pack4<FP8>(y, 0.0f, 0.0f, 0.0f));

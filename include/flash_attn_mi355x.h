@@ -393,8 +393,9 @@ int fa_decode_weighted_fp16(const void* q, const void* k, const void* v,
  *   block_table[b, t / page] (int32 [B, max_blocks]), row t % page.
  *   k_cache/v_cache [num_pages, H_KV, page, D]: int8 codes, or e4m3 with fp8;
  *   k_scale/v_scale fp32 [num_pages, H_KV]; page 16, 32, 64, 128 or 256.
- *   A value is code * scale; scale = max |x| / 127 (e4m3: 448) over the page's
- *   tokens of the head, code = x / scale rounded to nearest even.  In a page
+ *   A value is code * scale; scale = max |x| * (1 / 127) (e4m3: 1 / 448) over the
+ *   page's tokens of the head, code = x / scale rounded to nearest even, in fp32.
+ *   In a page
  *   that already holds tokens of the sequence the scale only grows, and where it
  *   does the old codes are rounded again.  Rows of a page that are neither new
  *   nor before the new ones are left as they are.  Tokens past the table row or

@@ -652,7 +652,7 @@ def append_paged_kv8(k, v, cu, lens, max_new, k_cache, v_cache, k_scale, v_scale
                 pg = int(table[b, at // page]) if at // page < table.shape[1] else -1
                 if 0 <= pg < pages:
                     x = new[lo + at - int(lens[b]):lo + upto - int(lens[b])].float().transpose(0, 1)
-                    scale = x.abs().amax((1, 2)) / torch.tensor(KV8_TOP[dtype])
+                    scale = x.abs().amax((1, 2)) * (torch.tensor(1.0) / torch.tensor(KV8_TOP[dtype]))
                     first = at % page
                     if first:
                         before = scales[pg]
