@@ -30,7 +30,7 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
 
 KERNEL_SOURCES = ["decode.hip", "prefill.hip", "train.hip", "train_fp32.hip", "token_ops.hip", "tp_ops.hip",
-                  "scored.hip", "scored_fp32.hip", "token_decode.hip", "kv_cache_ops.hip"]
+                  "scored.hip", "scored_backward.hip", "scored_fp32.hip", "token_decode.hip", "kv_cache_ops.hip"]
 HOST_SOURCES = ["capi.cpp"]
 
 HIP_FLAGS = [
@@ -46,7 +46,7 @@ HIP_FLAGS = [
 # stored) in AGPRs.
 VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 SOURCE_FLAGS = {"decode.hip": VGPR_FORM, "prefill.hip": VGPR_FORM, "train.hip": VGPR_FORM,
-                "scored.hip": VGPR_FORM, "token_decode.hip": VGPR_FORM}
+                "scored.hip": VGPR_FORM, "scored_backward.hip": VGPR_FORM, "token_decode.hip": VGPR_FORM}
 
 
 def _run(cmd):

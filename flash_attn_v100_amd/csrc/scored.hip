@@ -1,55 +1,16 @@
 // Attention with modified scores (tanh cap, distance bias, document and prefix
-// masks): C ABI, and the fp16 instantiations of the forward and backward
-// kernels (scored_kernels.h).
+// masks): C ABI, and the fp16 instantiations of the forward kernels
+// (scored_kernels.h).
 #include <math.h>
-
-#include <type_traits>
 
 #include "scored_launch.h"
 
 namespace fa {
 namespace scored {
 
-// fp16 shapes: padded width DP, computed columns DC, row mode.  Backward: D <= 128.
-template <bool BACKWARD, typename Run>
-static void by_shape(int D, bool vec, Run&& run) {
-  constexpr std::integral_constant<int, 64> w64;
-  constexpr std::integral_constant<int, 96> w96;
-  constexpr std::integral_constant<int, 128> w128;
-  constexpr std::integral_constant<int, kRowElems> elems;
-  constexpr std::integral_constant<int, kRowFull> full;
-  constexpr std::integral_constant<int, kRowChunks> chunks;
-  const bool v = vec && D % 8 == 0;
-  if constexpr (!BACKWARD) {
-    if (D > 128) {
-      constexpr std::integral_constant<int, 192> w192;
-      constexpr std::integral_constant<int, 256> w256;
-      if (!v) run(w256, w256, elems);
-      else if (D == 256) run(w256, w256, full);
-      else if (D <= 192) run(w256, w192, chunks);
-      else run(w256, w256, chunks);
-      return;
-    }
-  }
-  if (!v) {
-    if (D <= 64) run(w64, w64, elems);
-    else run(w128, w128, elems);
-  } else if (D == 64) run(w64, w64, full);
-  else if (D < 64) run(w64, w64, chunks);
-  else if (D <= 96) run(w128, w96, chunks);
-  else if (D == 128) run(w128, w128, full);
-  else run(w128, w128, chunks);
-}
-
 static void forward_fp16(const ScoredParams& p, bool vec, hipStream_t st) {
-  by_shape<false>(p.D, vec, [&](auto dp, auto dc, auto rows) {
-    launch_query<half_t, dp(), dc(), rows(), 0, kAnyMods>(p, split_query(p), st);
-  });
-}
-
-static void backward_fp16(const ScoredParams& p, bool vec, hipStream_t st) {
-  by_shape<true>(p.D, vec, [&](auto dp, auto dc, auto rows) {
-    launch_backward_shape<half_t, dp(), dc(), rows(), kAnyMods>(p, st);
+  by_shape_fp16<true>(p.D, vec, p.mods, [&](auto dp, auto dc, auto rows, auto mods) {
+    launch_query<half_t, dp(), dc(), rows(), 0, mods()>(p, split_query(p), st);
   });
 }
 

@@ -1,6 +1,7 @@
 // Device kernels of attention with modified scores for gfx950: forward (with
 // optional log-sum-exp) and backward (dQ, dK, dV), fp16 and fp32, grouped KV
-// heads.  Instantiated by scored.hip (fp16) and scored_fp32.hip.
+// heads.  Instantiated by scored.hip and scored_backward.hip (fp16) and
+// scored_fp32.hip.
 //
 //   s_ij   = q_i . k_j / sqrt(D)
 //   c_ij   = cap tanh(s_ij / cap)            (cap > 0; else s_ij)
@@ -118,73 +119,98 @@ __device__ __forceinline__ bool map_block(const ScoredParams& p, int heads, bool
 
 typedef int int4u __attribute__((ext_vector_type(4), aligned(4)));
 
+// Least and largest over the wave: lane permutes within the rows of 16, scalar
+// instructions over the four rows.
 __device__ __forceinline__ int wave_min_i(int x) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) x = min(x, __shfl_xor(x, off, 64));
-  return __builtin_amdgcn_readfirstlane(x);
+  x = min(x, dpp_mov_i<kDppQuadXor1>(x));
+  x = min(x, dpp_mov_i<kDppQuadXor2>(x));
+  x = min(x, dpp_mov_i<kDppRowHalfMirror>(x));
+  x = min(x, dpp_mov_i<kDppRowMirror>(x));
+  return min(min(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)),
+             min(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
 }
-__device__ __forceinline__ int wave_max_i(int x) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) x = max(x, __shfl_xor(x, off, 64));
-  return __builtin_amdgcn_readfirstlane(x);
-}
+__device__ __forceinline__ int wave_max_i(int x) { return -wave_min_i(-x); }
 
 constexpr int kMixedIds = -1;       // a sub-tile of several ids (or a ragged one)
-constexpr int kNoId = -2147483647;  // own rows that see nothing; differs from every staged id
+constexpr int kNoId = -2147483646;  // own rows that see nothing; differs from every staged id
 
 // The tiles a workgroup streams: SUBS 32-row sub-tiles each, `count` of them
 // from row `first`, last to first with `rev`.  With ids, only those that hold
-// an id of [lo, hi].
+// an id of [lo, hi], and the first in walk order where `own` says that it holds
+// the workgroup's own rows (its copies start before any id has arrived).
 template <int SUBS>
 struct TileWalk {
   const int32_t* ids;  // of the streamed rows' batch row, or null
   int rows, first, count, lo, hi;
-  bool rev;
+  bool rev, own;
   int vt = 0;          // without ids: next tile in walk order
-  int base = -64;      // with ids: first sub-tile (in walk order) of the group held
+  int base = 0;        // with ids: first sub-tile (in walk order) of the group held
   uint64_t live = 0, pads = 0;
   int uni = 0;         // this lane's sub-tile: its single id, or kMixedIds
   // the tile that next() gave
-  int tile = -1;
+  int tile = -1, at = 0;
   uint64_t cur_pads = 0;
 
-  __device__ __forceinline__ void scan() {
-    const int lane = threadIdx.x & 63;
-    const int v = base + lane;
-    const int t = v / SUBS;
-    int mn = 0x7fffffff, mx = -1;
-    bool pad = false, ragged = true;
-    if (t < count) {
-      const int r0 = first + ((rev ? count - 1 - t : t) * SUBS + v % SUBS) * kRows;
-      ragged = r0 + kRows > rows;
-      auto take = [&](int id) {
-        pad |= id < 0;
-        if (id >= 0) mn = min(mn, id);
-        mx = max(mx, id);
-      };
-      if (!ragged) {
-        int4u x[kRows / 4];
+  __device__ __forceinline__ int phys(int t) const { return rev ? count - 1 - t : t; }
+  // First row of this lane's sub-tile of the group, past the last row if it has none.
+  __device__ __forceinline__ int lane_row() const {
+    const int v = base + (threadIdx.x & 63);
+    return v / SUBS < count ? first + (phys(v / SUBS) * SUBS + v % SUBS) * kRows : rows;
+  }
+  typedef int4u Ids[kRows / 4];
+  // Issues the reads of the first group's ids ...
+  __device__ __forceinline__ void load(Ids& raw) const {
+    const int r0 = lane_row();
+    if (r0 + kRows <= rows) {
 #pragma unroll
-        for (int i = 0; i < kRows / 4; ++i) x[i] = *reinterpret_cast<const int4u*>(ids + r0 + 4 * i);
-#pragma unroll
-        for (int i = 0; i < kRows / 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) take(x[i][j]);
-      } else {
-        for (int r = r0; r < rows; ++r) take(ids[r]);
-      }
+      for (int i = 0; i < kRows / 4; ++i) raw[i] = *reinterpret_cast<const int4u*>(ids + r0 + 4 * i);
     }
-    uni = !ragged && !pad && mn == mx ? mn : kMixedIds;
+  }
+  // ... and turns them into its masks.
+  __device__ __forceinline__ void digest(const Ids& raw) {
+    masks([&](auto&& take) {
+#pragma unroll
+      for (int i = 0; i < kRows / 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) take(raw[i][j]);
+    });
+    if (own) live |= 1;
+  }
+  // A later group, in the loop: few registers rather than all reads at once.
+  __device__ __forceinline__ void scan() {
+    const int r0 = lane_row();
+    masks([&](auto&& take) {
+#pragma unroll 2
+      for (int i = 0; i < kRows / 4; ++i) {
+        const int4u x = *reinterpret_cast<const int4u*>(ids + r0 + 4 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) take(x[j]);
+      }
+    });
+  }
+  // The group's masks, from a whole sub-tile's ids as `whole` passes them on.
+  template <typename Whole>
+  __device__ __forceinline__ void masks(Whole&& whole) {
+    const int r0 = lane_row();
+    int mn = 0x7fffffff, mx = -1, least = 0;
+    auto take = [&](int id) {
+      least = min(least, id);
+      mn = min(mn, id < 0 ? 0x7fffffff : id);
+      mx = max(mx, id);
+    };
+    const bool full = r0 + kRows <= rows;
+    if (full) whole(take);
+    else for (int r = r0; r < rows; ++r) take(ids[r]);
+    uni = full && least >= 0 && mn == mx ? mn : kMixedIds;
     live = __builtin_amdgcn_ballot_w64(mx >= lo && mn <= hi && mn <= mx);
-    pads = __builtin_amdgcn_ballot_w64(pad);
+    pads = __builtin_amdgcn_ballot_w64(least < 0);
   }
   // Steps to the next tile; false when there is none.  Every lane of every
   // wave of the workgroup takes the same steps.
   __device__ __forceinline__ bool next() {
     if (ids == nullptr) {
       if (vt >= count) return false;
-      tile = rev ? count - 1 - vt : vt;
-      ++vt;
+      tile = phys(vt++);
       return true;
     }
     while (live == 0) {
@@ -196,12 +222,10 @@ struct TileWalk {
     const uint64_t mask = (SUBS == 1 ? 1ull : (1ull << SUBS) - 1) << bit;
     live &= ~mask;
     cur_pads = pads & mask;
-    const int v = (base + bit) / SUBS;
-    tile = rev ? count - 1 - v : v;
+    tile = phys((base + bit) / SUBS);
     at = bit;
     return true;
   }
-  int at = 0;
   // Single id of sub-tile `sub` of the current tile, or kMixedIds.
   __device__ __forceinline__ int sub_id(int sub) const { return __builtin_amdgcn_readlane(uni, at + sub); }
 };
@@ -242,19 +266,23 @@ __device__ __forceinline__ void add_bias(float16_t& y, float slope2, float rel) 
   for (int r = 0; r < 16; ++r) y[r] = fmaf(-slope2, fabsf(rel + static_cast<float>(8 * (r >> 2) + (r & 3))), y[r]);
 }
 
-// Ids of the 16 tile rows r0 + 8 (r / 4) + r % 4 (negative ones as -1), -1 past `rows`.
-__device__ __forceinline__ void load_ids(int (&id)[16], const int32_t* ids, int r0, int rows) {
+// Calls use(r, same) for the 16 tile rows r0 + 8 (r / 4) + r % 4: whether the row's id is `mine`
+// (an id >= 0, or one that no row has).
+template <typename Use>
+__device__ __forceinline__ void compare_ids(const int32_t* ids, int r0, int rows, int mine, Use&& use) {
 #pragma unroll
   for (int rr = 0; rr < 4; ++rr) {
     const int row = r0 + 8 * rr;
+    int4u x = {-1, -1, -1, -1};
     if (row + 4 <= rows) {
-      const int4u x = *reinterpret_cast<const int4u*>(ids + row);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) id[4 * rr + j] = max(x[j], -1);
+      x = *reinterpret_cast<const int4u*>(ids + row);
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) id[4 * rr + j] = row + j < rows ? max(ids[row + j], -1) : -1;
+      for (int j = 0; j < 4; ++j)
+        if (row + j < rows) x[j] = ids[row + j];
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) use(4 * rr + j, max(x[j], -1) == mine);
   }
 }
 
@@ -276,7 +304,8 @@ __device__ __forceinline__ void zero_pad_rows(const Ring& ring, int stage, const
 
 // Streams the walk's tiles through the ring, HEADS rounds a tile (key-major:
 // the query heads in turn), and calls compute(stage, tile, round, sub id) for
-// each; fetch(tile, round, stage) copies (DMA) or loads (registers) one.
+// each; fetch(tile, round, stage) copies (DMA) or loads (registers) one.  The
+// caller has fetched the first tile of a walk that starts at its own rows.
 template <typename T, typename Ring, bool DMA, int SUBS, typename Fetch, typename Compute>
 __device__ __forceinline__ void stream_tiles(Ring& ring, TileWalk<SUBS>& walk, int heads, int sub, int N, Fetch&& fetch,
                                              Compute&& compute) {
@@ -284,7 +313,7 @@ __device__ __forceinline__ void stream_tiles(Ring& ring, TileWalk<SUBS>& walk, i
   if (!more) return;
   int tile = walk.tile, id = walk.ids ? walk.sub_id(sub) : 0, head = 0, stage = 0;
   uint64_t pads = walk.cur_pads;
-  fetch(tile, 0, 0);
+  if (!walk.own) fetch(tile, 0, 0);
   if constexpr (!DMA) ring.store(0);
   for (;;) {
     // the (tile, head) after this one
@@ -321,8 +350,14 @@ __device__ __forceinline__ void stream_tiles(Ring& ring, TileWalk<SUBS>& walk, i
 
 // ---------------------------------------------------------------------------
 // Query-major kernel: MODE 0 = forward (O, optional LSE), MODE 1 = dQ + delta.
+// Registers: the fp16 forward asks for three waves per SIMD up to D = 128 (LDS allows
+// them in whole blocks), fp32 at D <= 64 for two.
+template <typename T, int DP, int MODE, int SPLIT, int MODS>
+constexpr int query_waves() {
+  return sizeof(T) == 4 ? (DP <= 64 ? 2 : 1) : (MODE == 0 && DP <= 128 && SPLIT == 1 && (MODS & kAnyMods) == 0 ? 3 : 1);
+}
 template <typename T, int DP, int DC, int ROWS, int MODE, int SPLIT, int MODS>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP <= 64 ? 2 : 1))) void scored_query_kernel(
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_waves<T, DP, MODE, SPLIT, MODS>()))) void scored_query_kernel(
     ScoredParams p) {
   typedef typename Elem<T>::frag F;
   constexpr int KK = DC / 16;
@@ -355,51 +390,88 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
   const T* __restrict__ vp = static_cast<const T*>(p.v) + kbase;
   const bool cap = has<MODS>(p, kCap), bias = has<MODS>(p, kBias), docs = has<MODS>(p, kDocs);
 
+  // keys every row sees, and the last key of this lane's row
+  const int pre = p.prefix != nullptr ? max(0, min(p.prefix[b], N)) : 0;
+  const int last = p.causal ? max(min(qrow, N - 1), pre - 1) : N - 1;
+  const int kend = p.causal ? max(min(N, q0 + RW * kRows), pre) : N;
+  const int kend_w = wq0 >= N ? 0 : (p.causal ? max(min(N, wq0 + kRows), pre) : N);
+  constexpr int SR = Ring::SR;
   TileWalk<SPLIT> walk;
   walk.ids = docs ? p.ids + static_cast<size_t>(b) * N : nullptr;
-  int my_id = 0, wlo = 0, whi = 0;
+  walk.rows = N;
+  walk.first = 0;
+  walk.count = (kend + SR - 1) / SR;
+  // With a bias the nearest keys weigh most: a causal walk that starts at the
+  // diagonal finds the running maximum at once.  With ids, the diagonal tile is
+  // sure to be needed.
+  walk.rev = p.causal && (bias || docs);
+  walk.own = docs && p.causal && pre == 0;
+
+  Ring ring(smem, tid, D);
+  auto fetch = [&](int tile, int, int stage) {
+    if constexpr (DMA) ring.dma(kp, vp, nullptr, nullptr, tile * SR, N, D, stage);
+    else ring.load(kp, vp, nullptr, nullptr, tile * SR, N, D);
+  };
+  // Every read that the walk waits for is issued here, before the first wait:
+  // ids, this lane's rows, the first tile.
+  int my_id = 0, wlo = 0, whi = 0, block_id[RW * kRows / 64];
+  typename TileWalk<SPLIT>::Ids group_ids;
   if (docs) {
+    walk.load(group_ids);
     my_id = qrow < N ? walk.ids[qrow] : -1;
+#pragma unroll
+    for (int i = 0; i < RW * kRows / 64; ++i) block_id[i] = q0 + lane + 64 * i < N ? walk.ids[q0 + lane + 64 * i] : -1;
+  }
+  // resident B operands: lane's query row, d = 16 kk + 8 hi .. +8
+  F qf[KK], df[KK], of[KK];
+  float lse2 = 0.0f, delta = 0.0f;
+  {
+    const size_t row = qbase + static_cast<size_t>(min(qrow, N - 1)) * D;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      qf[kk] = load_frag<T, ROWS>(static_cast<const T*>(p.q) + row, 16 * kk + 8 * hi, D);
+      if constexpr (MODE == 1) {
+        df[kk] = load_frag<T, ROWS>(static_cast<const T*>(p.dout) + row, 16 * kk + 8 * hi, D);
+        of[kk] = load_frag<T, ROWS>(static_cast<const T*>(p.o) + row, 16 * kk + 8 * hi, D);
+      }
+    }
+    if constexpr (MODE == 1) lse2 = p.lse[qhead * N + min(qrow, N - 1)] * kLog2e;
+  }
+  const float slope2 = bias ? p.slopes[h] * kLog2e : 0.0f;
+  if (walk.own) fetch(walk.phys(0), 0, 0);
+  if (docs) {
     my_id = my_id < 0 ? kNoId : my_id;
     wlo = wave_min_i(my_id < 0 ? 0x7fffffff : my_id);
     whi = wave_max_i(my_id);
-    int lo = 0x7fffffff, hi_ = -1;
-    for (int r = lane; r < RW * kRows; r += 64) {
-      const int id = q0 + r < N ? walk.ids[q0 + r] : -1;
-      if (id >= 0) lo = min(lo, id);
-      hi_ = max(hi_, id);
+    int lo = 0x7fffffff, top = -1;
+#pragma unroll
+    for (int i = 0; i < RW * kRows / 64; ++i) {
+      lo = min(lo, block_id[i] < 0 ? 0x7fffffff : block_id[i]);
+      top = max(top, block_id[i]);
     }
     walk.lo = wave_min_i(lo);
-    walk.hi = wave_max_i(hi_);
+    walk.hi = wave_max_i(top);
+    walk.digest(group_ids);
   }
   const bool live = qrow < N && my_id >= 0;  // this lane's row sees something
   // single id of the wave's rows, or none
   const int wid = docs && wlo == whi && __builtin_amdgcn_ballot_w64(my_id != whi) == 0 ? whi : kNoId;
-
-  // resident B operands: lane's query row, d = 16 kk + 8 hi .. +8
-  F qf[KK], df[KK];
-  float delta = 0.0f, lse2 = 0.0f;
-  {
-    const T* qr = static_cast<const T*>(p.q) + qbase + static_cast<size_t>(min(qrow, N - 1)) * D;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) qf[kk] = live ? load_frag<T, ROWS>(qr, 16 * kk + 8 * hi, D) : zero_frag<T>();
-  }
-  if constexpr (MODE == 1) {
-    const size_t row = qbase + static_cast<size_t>(min(qrow, N - 1)) * D;
-    const T* dr = static_cast<const T*>(p.dout) + row;
-    const T* orow = static_cast<const T*>(p.o) + row;
-    float part = 0.0f;
+  if (!live) {
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
-      df[kk] = live ? load_frag<T, ROWS>(dr, 16 * kk + 8 * hi, D) : zero_frag<T>();
-      const F of = live ? load_frag<T, ROWS>(orow, 16 * kk + 8 * hi, D) : zero_frag<T>();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) part = fmaf(static_cast<float>(df[kk][j]), static_cast<float>(of[j]), part);
+      qf[kk] = zero_frag<T>();
+      if constexpr (MODE == 1) df[kk] = of[kk] = zero_frag<T>();
     }
+  }
+  if constexpr (MODE == 1) {
+    float part = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part = fmaf(static_cast<float>(df[kk][j]), static_cast<float>(of[kk][j]), part);
     delta = part + __shfl_xor(part, 32, 64);
     if (qrow < N && hi == 0 && sub == 0) p.delta[qhead * N + qrow] = delta;
-    lse2 = live ? p.lse[qhead * N + qrow] * kLog2e : INFINITY;
-    if (lse2 == -INFINITY) lse2 = INFINITY;  // rows that see nothing: P = 0
+    if (!live || lse2 == -INFINITY) lse2 = INFINITY;  // rows that see nothing: P = 0
   }
 
   float16_t acc[DB];
@@ -409,28 +481,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
     for (int r = 0; r < 16; ++r) acc[db][r] = 0.0f;
   float m_run = kNegBig, l_run = 0.0f;  // forward only (log2 domain)
   const float c = cap || bias ? 1.0f : p.scale_log2;
-  const float slope2 = bias ? p.slopes[h] * kLog2e : 0.0f;
-
-  // keys every row sees, and the last key of this lane's row
-  const int pre = p.prefix != nullptr ? max(0, min(p.prefix[b], N)) : 0;
-  const int last = p.causal ? max(min(qrow, N - 1), pre - 1) : N - 1;
-  const int kend = p.causal ? max(min(N, q0 + RW * kRows), pre) : N;
-  const int kend_w = wq0 >= N ? 0 : (p.causal ? max(min(N, wq0 + kRows), pre) : N);
-  constexpr int SR = Ring::SR;
-  walk.rows = N;
-  walk.first = 0;
-  walk.count = (kend + SR - 1) / SR;
-  // With a bias the nearest keys weigh most: a causal walk that starts at the
-  // diagonal finds the running maximum at once.
-  walk.rev = bias && p.causal;
-
-  Ring ring(smem, tid, D);
   const Reader<T, DP> rd(lane);
   constexpr unsigned kSubBytes = kRows * Layout<T, DP>::LD * sizeof(T);
-  auto fetch = [&](int tile, int, int stage) {
-    if constexpr (DMA) ring.dma(kp, vp, nullptr, nullptr, tile * SR, N, D, stage);
-    else ring.load(kp, vp, nullptr, nullptr, tile * SR, N, D);
-  };
   stream_tiles<T, Ring, DMA, SPLIT>(ring, walk, 1, sub, N, fetch, [&](int stage, int tile, int, int id) {
     const int kt = tile * SR + sub * kRows;
     if (kt >= kend_w) return;                               // past this wave's rows
@@ -471,10 +523,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = my_id == id ? s[r] : -INFINITY;
       } else {
-        int key_id[16];
-        load_ids(key_id, walk.ids, kt + 4 * hi, N);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = my_id == key_id[r] ? s[r] : -INFINITY;
+        compare_ids(walk.ids, kt + 4 * hi, N, my_id, [&](int r, bool same) { s[r] = same ? s[r] : -INFINITY; });
       }
     }
     float16_t pm;  // P^T (forward) or dS^T (dQ)
@@ -629,35 +678,72 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
   const size_t qhead0 = static_cast<size_t>(b) * p.H_Q + static_cast<size_t>(hk) * p.G;  // first query head of the group
   const bool cap = has<MODS>(p, kCap), bias = has<MODS>(p, kBias), docs = has<MODS>(p, kDocs);
 
+  const int pre = p.prefix != nullptr ? max(0, min(p.prefix[b], N)) : 0;
+  // causal: rows before the first key see it only inside the prefix
+  const int qstart = p.causal && k0 >= pre ? k0 : 0;
+  constexpr int SR = Ring::SR;
   TileWalk<SPLIT> walk;
   walk.ids = docs ? p.ids + static_cast<size_t>(b) * N : nullptr;
-  int my_id = 0, wlo = 0, whi = 0;
-  if (docs) {
-    my_id = krow < N ? walk.ids[krow] : -1;
-    my_id = my_id < 0 ? kNoId : my_id;
-    wlo = wave_min_i(my_id < 0 ? 0x7fffffff : my_id);
-    whi = wave_max_i(my_id);
-    int lo = 0x7fffffff, hi_ = -1;
-    for (int r = lane; r < RW * kRows; r += 64) {
-      const int id = k0 + r < N ? walk.ids[k0 + r] : -1;
-      if (id >= 0) lo = min(lo, id);
-      hi_ = max(hi_, id);
-    }
-    walk.lo = wave_min_i(lo);
-    walk.hi = wave_max_i(hi_);
-  }
-  const bool live = krow < N && my_id >= 0;
-  const int wid = docs && wlo == whi && __builtin_amdgcn_ballot_w64(my_id != whi) == 0 ? whi : kNoId;
+  walk.rows = N;
+  walk.first = qstart;
+  walk.count = (N - qstart + SR - 1) / SR;
+  // causal blocks of a head all end at the last query tile: walking backwards
+  // they read each tile at about the same time and share it through L2.  With
+  // ids, the first tile is the diagonal one, sure to be needed.
+  walk.rev = p.causal != 0 && !docs;
+  walk.own = docs && p.causal && qstart == k0;
 
+  Ring ring(smem, tid, D);
+  auto fetch = [&](int tile, int g, int stage) {
+    const size_t head = qhead0 + g;
+    const T* qp = static_cast<const T*>(p.q) + head * N * D;
+    const T* dp = static_cast<const T*>(p.dout) + head * N * D;
+    const float* lse = p.lse + head * N;
+    // the dV pass never reads delta: lse stands in for it in its stream
+    const float* second = DO_DK ? p.delta + head * N : lse;
+    if constexpr (DMA) ring.dma(qp, dp, lse, second, qstart + tile * SR, N, D, stage);
+    else ring.load(qp, dp, lse, second, qstart + tile * SR, N, D);
+  };
+  // every read that the walk waits for, before the first wait
+  int my_id = 0, wlo = 0, whi = 0, block_id[RW * kRows / 64];
+  typename TileWalk<SPLIT>::Ids group_ids;
+  if (docs) {
+    walk.load(group_ids);
+    my_id = krow < N ? walk.ids[krow] : -1;
+#pragma unroll
+    for (int i = 0; i < RW * kRows / 64; ++i) block_id[i] = k0 + lane + 64 * i < N ? walk.ids[k0 + lane + 64 * i] : -1;
+  }
   F kf[KK], vf[KK];
   {
     const size_t row = kbase + static_cast<size_t>(min(krow, N - 1)) * D;
-    const T* kr = static_cast<const T*>(p.k) + row;
-    const T* vr = static_cast<const T*>(p.v) + row;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
-      kf[kk] = live ? load_frag<T, ROWS>(kr, 16 * kk + 8 * hi, D) : zero_frag<T>();
-      if constexpr (DO_DK) vf[kk] = live ? load_frag<T, ROWS>(vr, 16 * kk + 8 * hi, D) : zero_frag<T>();
+      kf[kk] = load_frag<T, ROWS>(static_cast<const T*>(p.k) + row, 16 * kk + 8 * hi, D);
+      if constexpr (DO_DK) vf[kk] = load_frag<T, ROWS>(static_cast<const T*>(p.v) + row, 16 * kk + 8 * hi, D);
+    }
+  }
+  if (walk.own) fetch(0, 0, 0);
+  if (docs) {
+    my_id = my_id < 0 ? kNoId : my_id;
+    wlo = wave_min_i(my_id < 0 ? 0x7fffffff : my_id);
+    whi = wave_max_i(my_id);
+    int lo = 0x7fffffff, top = -1;
+#pragma unroll
+    for (int i = 0; i < RW * kRows / 64; ++i) {
+      lo = min(lo, block_id[i] < 0 ? 0x7fffffff : block_id[i]);
+      top = max(top, block_id[i]);
+    }
+    walk.lo = wave_min_i(lo);
+    walk.hi = wave_max_i(top);
+    walk.digest(group_ids);
+  }
+  const bool live = krow < N && my_id >= 0;
+  const int wid = docs && wlo == whi && __builtin_amdgcn_ballot_w64(my_id != whi) == 0 ? whi : kNoId;
+  if (!live) {
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      kf[kk] = zero_frag<T>();
+      if constexpr (DO_DK) vf[kk] = zero_frag<T>();
     }
   }
   float16_t dk[DB], dv[DB];
@@ -669,32 +755,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
       dv[db][r] = 0.0f;
     }
   const float c = cap || bias ? 1.0f : p.scale_log2;
-  const int pre = p.prefix != nullptr ? max(0, min(p.prefix[b], N)) : 0;
-  // causal: rows before the first key see it only inside the prefix
-  const int qstart = p.causal && k0 >= pre ? k0 : 0;
-  constexpr int SR = Ring::SR;
-  walk.rows = N;
-  walk.first = qstart;
-  walk.count = (N - qstart + SR - 1) / SR;
-  // causal blocks of a head all end at the last query tile: walking backwards
-  // they read each tile at about the same time and share it through L2
-  walk.rev = p.causal != 0 && !docs;
   const bool every = !p.causal || wk0 + kRows <= pre;  // every query sees the wave's keys
   const int key_from = p.causal && krow >= pre ? krow : 0;
 
-  Ring ring(smem, tid, D);
   const Reader<T, DP> rd(lane);
   constexpr unsigned kSubBytes = kRows * Layout<T, DP>::LD * sizeof(T);
-  auto fetch = [&](int tile, int g, int stage) {
-    const size_t head = qhead0 + g;
-    const T* qp = static_cast<const T*>(p.q) + head * N * D;
-    const T* dp = static_cast<const T*>(p.dout) + head * N * D;
-    const float* lse = p.lse + head * N;
-    // the dV pass never reads delta: lse stands in for it in its stream
-    const float* second = DO_DK ? p.delta + head * N : lse;
-    if constexpr (DMA) ring.dma(qp, dp, lse, second, qstart + tile * SR, N, D, stage);
-    else ring.load(qp, dp, lse, second, qstart + tile * SR, N, D);
-  };
   stream_tiles<T, Ring, DMA, SPLIT>(ring, walk, p.G, sub, N, fetch, [&](int stage, int tile, int g, int id) {
     const int qt = qstart + tile * SR + sub * kRows;
     if (qt >= N || wk0 >= N) return;
@@ -772,10 +837,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
 #pragma unroll
         for (int r = 0; r < 16; ++r) keep(r, my_id == id);
       } else {
-        int row_id[16];
-        load_ids(row_id, walk.ids, qt + 4 * hi, N);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) keep(r, my_id == row_id[r]);
+        compare_ids(walk.ids, qt + 4 * hi, N, my_id, keep);
       }
     }
     if constexpr (DO_DV) {

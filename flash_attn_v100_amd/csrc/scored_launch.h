@@ -3,6 +3,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "capi_internal.h"
 #include "scored_kernels.h"
@@ -83,7 +84,58 @@ void launch_backward_shape(const ScoredParams& p, hipStream_t st) {
   }
 }
 
-// Entry points of the fp32 translation unit.
+// Calls run with the variant of the call's modifications: those met in practice
+// have one of their own, what is left reads them from the parameters.
+// Compiled in, prefill [1,32:8,8192,128] with a cap takes @A us for @B, a training
+// layer of documents [4,32:8,2048,128] @C for @D.
+template <typename Run>
+void by_mods(int mods, Run&& run) {
+  switch (mods) {
+    case 0: run(std::integral_constant<int, 0>()); break;
+    case kCap: run(std::integral_constant<int, kCap>()); break;
+    case kBias: run(std::integral_constant<int, kBias>()); break;
+    case kDocs: run(std::integral_constant<int, kDocs>()); break;
+    case kCap | kDocs: run(std::integral_constant<int, kCap | kDocs>()); break;
+    case kBias | kDocs: run(std::integral_constant<int, kBias | kDocs>()); break;
+    default: run(std::integral_constant<int, kAnyMods>());
+  }
+}
+
+// fp16 shapes: padded width DP, computed columns DC, row mode (elems: no vector
+// rows, and every modification read from the parameters).  WIDE: D up to 256.
+template <bool WIDE, typename Run>
+void by_shape_fp16(int D, bool vec, int mods, Run&& run) {
+  constexpr std::integral_constant<int, 64> w64;
+  constexpr std::integral_constant<int, 96> w96;
+  constexpr std::integral_constant<int, 128> w128;
+  constexpr std::integral_constant<int, 192> w192;
+  constexpr std::integral_constant<int, 256> w256;
+  constexpr std::integral_constant<int, kRowElems> elems;
+  constexpr std::integral_constant<int, kRowFull> full;
+  constexpr std::integral_constant<int, kRowChunks> chunks;
+  constexpr std::integral_constant<int, kAnyMods> any;
+  if (!vec || D % 8 != 0) {
+    if (D <= 64) run(w64, w64, elems, any);
+    else if (D <= 128) run(w128, w128, elems, any);
+    else if constexpr (WIDE) run(w256, w256, elems, any);
+    return;
+  }
+  by_mods(mods, [&](auto m) {
+    if (D == 64) run(w64, w64, full, m);
+    else if (D < 64) run(w64, w64, chunks, m);
+    else if (D <= 96) run(w128, w96, chunks, m);
+    else if (D == 128) run(w128, w128, full, m);
+    else if (D < 128) run(w128, w128, chunks, m);
+    else if constexpr (WIDE) {
+      if (D == 256) run(w256, w256, full, m);
+      else if (D <= 192) run(w256, w192, chunks, m);
+      else run(w256, w256, chunks, m);
+    }
+  });
+}
+
+// Entry points of the other translation units.
+void backward_fp16(const ScoredParams& p, bool vec, hipStream_t st);
 void forward_fp32(const ScoredParams& p, bool vec, hipStream_t st);
 void backward_fp32(const ScoredParams& p, bool vec, hipStream_t st);
 
