@@ -7,6 +7,7 @@ scores (forward_scored_with_lse, backward_scored)."""
 import torch
 
 import flash_attn_v100
+from flash_attn_v100_amd import _ext
 
 
 class FlashAttentionFunction(torch.autograd.Function):
@@ -34,29 +35,9 @@ def flash_attn(q, k, v, causal=True):
     return FlashAttentionFunction.apply(q, k, v, causal)
 
 
-class ScoredAttentionFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, causal, softcap, slopes, doc_ids, prefix_lens):
-        if slopes is not None and slopes.requires_grad:
-            raise RuntimeError("flash_attn_scored: slopes are constants of the gradient; detach them")
-        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
-        out, lse = flash_attn_v100.forward_scored_with_lse(q, k, v, causal, softcap, slopes, doc_ids, prefix_lens)
-        ctx.save_for_backward(q, k, v, out, lse, slopes, doc_ids, prefix_lens)
-        ctx.args = causal, softcap
-        return out
-
-    @staticmethod
-    def backward(ctx, dout):
-        q, k, v, out, lse, slopes, doc_ids, prefix_lens = ctx.saved_tensors
-        causal, softcap = ctx.args
-        dq, dk, dv = flash_attn_v100.backward_scored(dout.contiguous(), q, k, v, out, lse, causal, softcap, slopes,
-                                                     doc_ids, prefix_lens)
-        return dq, dk, dv, None, None, None, None, None
-
-
 def flash_attn_scored(q, k, v, causal=True, softcap=0.0, slopes=None, doc_ids=None, prefix_lens=None):
     """Attention of q [B, H_Q, N, D] over k, v [B, H_KV, N, D] (fp16 or fp32, D <= 128) whose scores are capped
     (``softcap * tanh(s / softcap)``), biased (``- slopes[h] * |i - j|``) and masked: causally, by document
     (``doc_ids`` int32 [B, N], equal ids see each other, negative ones nothing) and with a prefix every row sees
     (``prefix_lens`` int32 [B]).  Gradients for q, k and v."""
-    return ScoredAttentionFunction.apply(q, k, v, causal, softcap, slopes, doc_ids, prefix_lens)
+    return _ext._scored_autograd(q, k, v, causal, softcap, slopes, doc_ids, prefix_lens)

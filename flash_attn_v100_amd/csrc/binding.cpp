@@ -670,7 +670,7 @@ const T* optional_ptr(const OptTensor& x, const at::Tensor& q, const char* name,
 
 void check_softcap(double softcap) {
   const float cap = static_cast<float>(softcap);
-  TORCH_CHECK(cap == 0.0f || (cap >= 1e-3f && cap <= 1e6f), "softcap must be 0 (none) or lie in [1e-3, 1e6]");
+  TORCH_CHECK(cap == 0.0f || (cap >= 1e-2f && cap <= 1e3f), "softcap must be 0 (none) or lie in [0.01, 1000]");
 }
 
 struct ScoredArgs {
@@ -760,6 +760,42 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> backward_scored(at::Tensor dout, 
               dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), b, hq, hkv, n, d, causal ? 1 : 0, static_cast<float>(softcap),
               a.slopes, a.ids, a.prefix, ws_ptr(ws), bytes, cur_stream()));
   return std::make_tuple(dq, dk, dv);
+}
+
+// forward_scored_with_lse and backward_scored as one differentiable function.  In C++, so
+// that the autograd engine's thread does not wait for the interpreter: a step of a few
+// short kernels takes @F us, with a Python function @G.
+struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, at::Tensor q, at::Tensor k, at::Tensor v, bool causal,
+                            double softcap, OptTensor slopes, OptTensor doc_ids, OptTensor prefix_lens) {
+    q = q.contiguous();
+    k = k.contiguous();
+    v = v.contiguous();
+    auto [out, lse] = scored_impl(q, k, v, causal, softcap, slopes, doc_ids, prefix_lens, true);
+    auto some = [](const OptTensor& x) { return x.has_value() ? *x : at::Tensor(); };
+    ctx->save_for_backward({q, k, v, out, lse, some(slopes), some(doc_ids), some(prefix_lens)});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["softcap"] = softcap;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    auto opt = [](const at::Tensor& x) { return x.defined() ? OptTensor(x) : OptTensor(); };
+    auto [dq, dk, dv] =
+        backward_scored(grads[0].contiguous(), saved[0], saved[1], saved[2], saved[3], saved[4],
+                        ctx->saved_data["causal"].toBool(), ctx->saved_data["softcap"].toDouble(), opt(saved[5]),
+                        opt(saved[6]), opt(saved[7]));
+    const at::Tensor none;
+    return {dq, dk, dv, none, none, none, none, none};
+  }
+};
+
+at::Tensor scored_autograd(at::Tensor q, at::Tensor k, at::Tensor v, bool causal, double softcap, OptTensor slopes,
+                           OptTensor doc_ids, OptTensor prefix_lens) {
+  TORCH_CHECK(!slopes.has_value() || !slopes->requires_grad(),
+              "flash_attn_scored: slopes are constants of the gradient; detach them");
+  return ScoredAttention::apply(q, k, v, causal, softcap, slopes, doc_ids, prefix_lens);
 }
 
 // ---------------------------------------------------------------------------
@@ -1264,6 +1300,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("forward_scored_with_lse", &forward_scored_with_lse, "forward_scored with logsumexp (MI355X MFMA)", py::arg("q"),
         py::arg("k"), py::arg("v"), py::arg("causal"), py::arg("softcap") = 0.0, py::arg("slopes") = py::none(),
         py::arg("doc_ids") = py::none(), py::arg("prefix_lens") = py::none());
+  m.def("_scored_autograd", &scored_autograd);
   m.def("backward_scored", &backward_scored, "Backward of forward_scored_with_lse (MI355X MFMA)", py::arg("dout"),
         py::arg("q"), py::arg("k"), py::arg("v"), py::arg("out"), py::arg("logsumexp"), py::arg("causal"),
         py::arg("softcap") = 0.0, py::arg("slopes") = py::none(), py::arg("doc_ids") = py::none(),

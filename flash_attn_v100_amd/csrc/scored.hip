@@ -10,7 +10,7 @@ namespace scored {
 
 static void forward_fp16(const ScoredParams& p, bool vec, hipStream_t st) {
   by_shape_fp16<true>(p.D, vec, p.mods, [&](auto dp, auto dc, auto rows, auto mods) {
-    launch_query<half_t, dp(), dc(), rows(), 0, mods()>(p, split_query(p), st);
+    launch_query<half_t, dp(), dc(), rows(), 0, mods()>(p, split_query(p, false), st);
   });
 }
 
@@ -23,13 +23,13 @@ static int fill(const char* fn, ScoredParams& p, int B, int H_Q, int H_KV, int N
   if (H_Q < H_KV || H_Q % H_KV != 0)
     return set_error(FA_ERR_INVALID_ARG, "%s: H_Q (%d) must be a multiple of H_KV (%d)", fn, H_Q, H_KV);
   if (D > max_d) return set_error(FA_ERR_UNSUPPORTED, "%s: D=%d exceeds %d", fn, D, max_d);
-  // (the range keeps scale / softcap and its squares normal numbers)
-  if (softcap != 0.0f && !(softcap >= 1e-3f && softcap <= 1e6f))
-    return set_error(FA_ERR_INVALID_ARG, "%s: softcap must be 0 (none) or lie in [1e-3, 1e6]", fn);
+  // (the range keeps the polynomial's coefficients, up to (scale / softcap)^8, in fp32's)
+  if (softcap != 0.0f && !(softcap >= 1e-2f && softcap <= 1e3f))
+    return set_error(FA_ERR_INVALID_ARG, "%s: softcap must be 0 (none) or lie in [0.01, 1000]", fn);
   if (prefix != nullptr && !causal)
     return set_error(FA_ERR_INVALID_ARG, "%s: prefix lengths need a causal mask", fn);
-  // half-block workgroups of the padded units (deal)
-  if ((static_cast<long long>(B) * H_Q + 8 * kXcds * (H_Q / H_KV)) * (2LL * ceil_div(N, kBlockRows)) > 0x3fffffffLL)
+  // quarter-block workgroups of the padded units (deal)
+  if ((static_cast<long long>(B) * H_Q + 8 * kXcds * (H_Q / H_KV)) * (4LL * ceil_div(N, kBlockRows)) > 0x3fffffffLL)
     return set_error(FA_ERR_UNSUPPORTED, "%s: problem too large for one launch", fn);
   p.slopes = slopes;
   p.ids = ids;
@@ -41,6 +41,14 @@ static int fill(const char* fn, ScoredParams& p, int B, int H_Q, int H_KV, int N
   p.scale_log2 = p.scale * kLog2e;
   p.cap_in = softcap > 0.0f ? p.scale / softcap : 0.0f;
   p.cap_log2 = softcap * kLog2e;
+  if (softcap > 0.0f) {
+    const double in = static_cast<double>(p.scale) / softcap, in2 = in * in;
+    const double series[5] = {1.0, kTanhP0, kTanhP1, kTanhP2, kTanhP3};
+    double power = static_cast<double>(p.scale) * 1.4426950408889634;
+    for (int i = 0; i < 5; ++i, power *= in2) p.cap_poly[i] = static_cast<float>(series[i] * power);
+    p.cap_near = static_cast<float>(kTanhMax / in);
+    p.cap_slope = 1.0f / (p.cap_log2 * p.cap_log2);
+  }
   return FA_OK;
 }
 

@@ -8,7 +8,7 @@ namespace scored {
 
 template <int DP, int DC, int ROWS>
 static void forward_shape(const ScoredParams& p, hipStream_t st) {
-  launch_query<float, DP, DC, ROWS, 0, kAnyMods>(p, split_query(p), st);
+  launch_query<float, DP, DC, ROWS, 0, kAnyMods>(p, split_query(p, false), st);
 }
 
 template <typename Run>

@@ -80,6 +80,9 @@ struct ScoredParams {
   float scale_log2;       // scale * log2(e)
   float cap_in;           // scale / cap
   float cap_log2;         // cap * log2(e)
+  float cap_slope;        // 1 / cap_log2^2
+  float cap_near;         // raw products up to which the tanh's polynomial serves
+  float cap_poly[5];      // its coefficients
 };
 
 template <int MODS>
@@ -131,17 +134,34 @@ __device__ __forceinline__ int wave_min_i(int x) {
 }
 __device__ __forceinline__ int wave_max_i(int x) { return -wave_min_i(-x); }
 
+// Columns d0 .. d0 + 3 of an output row (d0 a multiple of 4; rows of whole 8-element
+// chunks hold all four or none of them).
+template <typename T, int ROWS>
+__device__ __forceinline__ void store4(T* row, int d0, int d, float a, float b, float c, float e) {
+  typedef T vec4 __attribute__((ext_vector_type(4)));
+  const vec4 x = {static_cast<T>(a), static_cast<T>(b), static_cast<T>(c), static_cast<T>(e)};
+  if constexpr (ROWS == kRowElems) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (d0 + j < d) row[d0 + j] = x[j];
+  } else {
+    if (ROWS == kRowFull || d0 < d) *reinterpret_cast<vec4*>(row + d0) = x;
+  }
+}
+
 constexpr int kMixedIds = -1;       // a sub-tile of several ids (or a ragged one)
 constexpr int kNoId = -2147483646;  // own rows that see nothing; differs from every staged id
 
 // The tiles a workgroup streams: SUBS 32-row sub-tiles each, `count` of them
-// from row `first`, last to first with `rev`.  With ids, only those that hold
-// an id of [lo, hi], and the first in walk order where `own` says that it holds
-// the workgroup's own rows (its copies start before any id has arrived).
+// from row `first`, last to first with `rev`, else from tile `start` on and
+// round to it.  With ids, only those that hold an id of [lo, hi], and the first in
+// walk order where `own` says that it holds the workgroup's own rows (its copies
+// start before any id has arrived).
 template <int SUBS>
 struct TileWalk {
   const int32_t* ids;  // of the streamed rows' batch row, or null
   int rows, first, count, lo, hi;
+  int start = 0;
   bool rev, own;
   int vt = 0;          // without ids: next tile in walk order
   int base = 0;        // with ids: first sub-tile (in walk order) of the group held
@@ -151,7 +171,10 @@ struct TileWalk {
   int tile = -1, at = 0;
   uint64_t cur_pads = 0;
 
-  __device__ __forceinline__ int phys(int t) const { return rev ? count - 1 - t : t; }
+  __device__ __forceinline__ int phys(int t) const {
+    if (rev) return count - 1 - t;
+    return t + start < count ? t + start : t + start - count;
+  }
   // First row of this lane's sub-tile of the group, past the last row if it has none.
   __device__ __forceinline__ int lane_row() const {
     const int v = base + (threadIdx.x & 63);
@@ -232,31 +255,24 @@ struct TileWalk {
 
 // ---- scores ----
 // Raw products s -> capped scores in the log2 domain, cap log2(e) tanh(s scale / cap).
-// Where every |z| of the wave's tile is at most 1/2 (scores below half the
-// cap) the polynomial serves: 8 full-rate operations a score where the
-// exponential form needs two quarter-rate ones more.
+// Where every score of the wave's tile is at most half the cap, tanh is the odd
+// polynomial of common.h with the scales folded into its coefficients, y = s (c0 +
+// c1 s^2 + ...): 6 full-rate operations a score, where the exponential form takes two
+// quarter-rate ones and 9 others.  (These kernels are bound by their vector
+// instructions: with the coefficients unfolded, 9 a score, @E.)
 __device__ __forceinline__ void cap_scores(float16_t& s, const ScoredParams& p) {
-  float16_t z;
   float big = 0.0f;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    z[r] = s[r] * p.cap_in;
-    big = fmaxf(big, fabsf(z[r]));
-  }
-  const bool far = __builtin_amdgcn_ballot_w64(!(big <= kTanhMax)) != 0;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const float w = z[r] * z[r];
-    const float zc = z[r] * p.cap_log2;
-    s[r] = fmaf(zc * w, tanh_p(w), zc);
-  }
-  if (far) {
+  for (int r = 0; r < 16; r += 2) big = fmaxf(fmaxf(fabsf(s[r]), fabsf(s[r + 1])), big);
+  if (__builtin_amdgcn_ballot_w64(!(big <= p.cap_near)) == 0) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const float y = __builtin_copysignf(tanh_far(z[r]) * p.cap_log2, z[r]);
-      s[r] = fabsf(z[r]) <= kTanhMax ? s[r] : y;
-      // (NaN compares false and comes through the exponential)
+      const float w = s[r] * s[r];
+      s[r] *= fmaf(fmaf(fmaf(fmaf(p.cap_poly[4], w, p.cap_poly[3]), w, p.cap_poly[2]), w, p.cap_poly[1]), w, p.cap_poly[0]);
     }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = tanh_f32(s[r] * p.cap_in) * p.cap_log2;
   }
 }
 
@@ -266,36 +282,49 @@ __device__ __forceinline__ void add_bias(float16_t& y, float slope2, float rel) 
   for (int r = 0; r < 16; ++r) y[r] = fmaf(-slope2, fabsf(rel + static_cast<float>(8 * (r >> 2) + (r & 3))), y[r]);
 }
 
-// Calls use(r, same) for the 16 tile rows r0 + 8 (r / 4) + r % 4: whether the row's id is `mine`
+// Ids of the staged tiles' rows, beside the ring: they travel with the tile, so
+// that a tile of several documents waits for nothing of its own (read from
+// global memory where a tile needs them, they drained the copies in flight: @H).
+constexpr int kStagedIds = kWaves * kRows;  // rows of a stage, at most
+
+// Fetches the ids of rows [r0, r0 + SR) (past `rows`: the last row's) into a stage's slots.
+template <int SR, bool DMA>
+__device__ __forceinline__ void fetch_ids(const int32_t* ids, int r0, int rows, int (&slots)[kStagedIds]) {
+  const int row = min(static_cast<int>(threadIdx.x) & (SR - 1), rows - 1 - r0);
+  if constexpr (DMA) {
+    // 64 slots a wave; of 32-row tiles half of them are used
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (64 * wave < SR)
+      copy4_to_lds(reinterpret_cast<const float*>(ids + r0), static_cast<unsigned>(row) * 4,
+                   static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) int*)slots)) + wave * 256);
+  } else {
+    if (threadIdx.x < SR) slots[threadIdx.x] = ids[r0 + row];
+  }
+}
+
+// Calls use(r, same) for the 16 tile rows 8 (r / 4) + r % 4 from `at`: whether the row's id is `mine`
 // (an id >= 0, or one that no row has).
 template <typename Use>
-__device__ __forceinline__ void compare_ids(const int32_t* ids, int r0, int rows, int mine, Use&& use) {
+__device__ __forceinline__ void compare_ids(const int* at, int mine, Use&& use) {
 #pragma unroll
   for (int rr = 0; rr < 4; ++rr) {
-    const int row = r0 + 8 * rr;
-    int4u x = {-1, -1, -1, -1};
-    if (row + 4 <= rows) {
-      x = *reinterpret_cast<const int4u*>(ids + row);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (row + j < rows) x[j] = ids[row + j];
-    }
+    typedef int int4a __attribute__((ext_vector_type(4)));
+    const int4a x = *reinterpret_cast<const int4a*>(at + 8 * rr);
 #pragma unroll
     for (int j = 0; j < 4; ++j) use(4 * rr + j, max(x[j], -1) == mine);
   }
 }
 
-// Zeroes the rows of negative id in the staged tile pair of rows [r0, r0 + SR)
-// (rows past `rows` may hold the last one again).
+// Zeroes the rows of negative id in the staged tile pair (rows past the last may
+// hold it again, with its id).
 template <typename T, typename Ring>
-__device__ __forceinline__ void zero_pad_rows(const Ring& ring, int stage, const int32_t* ids, int r0, int rows) {
+__device__ __forceinline__ void zero_pad_rows(const Ring& ring, int stage, const int* ids) {
   lds_ptr<T> ta = ring.tile_a(stage);
   lds_ptr<T> tb = ring.tile_b(stage);
   typedef typename Elem<T>::frag F;
   for (int c = threadIdx.x; c < Ring::CHUNKS; c += kThreads) {
     const int row = c / Ring::CPR, col = c % Ring::CPR * 8;
-    if (ids[min(r0 + row, rows - 1)] < 0) {
+    if (ids[row] < 0) {
       *reinterpret_cast<__attribute__((address_space(3))) F*>(ta + Ring::L::off(row, col)) = zero_frag<T>();
       *reinterpret_cast<__attribute__((address_space(3))) F*>(tb + Ring::L::off(row, col)) = zero_frag<T>();
     }
@@ -307,8 +336,8 @@ __device__ __forceinline__ void zero_pad_rows(const Ring& ring, int stage, const
 // each; fetch(tile, round, stage) copies (DMA) or loads (registers) one.  The
 // caller has fetched the first tile of a walk that starts at its own rows.
 template <typename T, typename Ring, bool DMA, int SUBS, typename Fetch, typename Compute>
-__device__ __forceinline__ void stream_tiles(Ring& ring, TileWalk<SUBS>& walk, int heads, int sub, int N, Fetch&& fetch,
-                                             Compute&& compute) {
+__device__ __forceinline__ void stream_tiles(Ring& ring, TileWalk<SUBS>& walk, int heads, int sub,
+                                             const int (&ids)[2][kStagedIds], Fetch&& fetch, Compute&& compute) {
   bool more = walk.next();
   if (!more) return;
   int tile = walk.tile, id = walk.ids ? walk.sub_id(sub) : 0, head = 0, stage = 0;
@@ -333,7 +362,7 @@ __device__ __forceinline__ void stream_tiles(Ring& ring, TileWalk<SUBS>& walk, i
       __syncthreads();
     }
     if (pads != 0) {
-      zero_pad_rows<T>(ring, stage, walk.ids, walk.first + tile * SUBS * kRows, N);
+      zero_pad_rows<T>(ring, stage, ids[stage]);
       __syncthreads();
     }
     if (more) fetch(ntile, nhead, stage ^ 1);
@@ -350,14 +379,16 @@ __device__ __forceinline__ void stream_tiles(Ring& ring, TileWalk<SUBS>& walk, i
 
 // ---------------------------------------------------------------------------
 // Query-major kernel: MODE 0 = forward (O, optional LSE), MODE 1 = dQ + delta.
-// Registers: the fp16 forward asks for three waves per SIMD up to D = 128 (LDS allows
-// them in whole blocks), fp32 at D <= 64 for two.
-template <typename T, int DP, int MODE, int SPLIT, int MODS>
+// Registers: the fp16 forward asks for three waves per SIMD up to D = 128, four up to
+// 96 (LDS allows them in whole blocks), fp32 at D <= 64 for two.
+template <typename T, int DC, int MODE, int SPLIT, int MODS>
 constexpr int query_waves() {
-  return sizeof(T) == 4 ? (DP <= 64 ? 2 : 1) : (MODE == 0 && DP <= 128 && SPLIT == 1 && (MODS & kAnyMods) == 0 ? 3 : 1);
+  if (sizeof(T) == 4) return DC <= 64 && SPLIT <= 2 ? 2 : 1;
+  if (MODE != 0 || DC > 128 || SPLIT > 1 || (MODS & kAnyMods) != 0) return 1;
+  return DC <= 96 && (MODS & kDocs) == 0 ? 4 : 3;
 }
 template <typename T, int DP, int DC, int ROWS, int MODE, int SPLIT, int MODS>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_waves<T, DP, MODE, SPLIT, MODS>()))) void scored_query_kernel(
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_waves<T, DC, MODE, SPLIT, MODS>()))) void scored_query_kernel(
     ScoredParams p) {
   typedef typename Elem<T>::frag F;
   constexpr int KK = DC / 16;
@@ -366,6 +397,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
   constexpr int RW = kWaves / SPLIT;  // 32-row blocks per workgroup
   typedef TileRing<T, DP, DMA, false, kRows * SPLIT, ROWS> Ring;
   __shared__ __attribute__((aligned(1024))) char smem[Ring::BYTES];
+  __shared__ __attribute__((aligned(16))) int s_ids[2][kStagedIds];
 
   const int N = p.N, D = p.D;
   int u, hg, blk;
@@ -401,26 +433,31 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
   walk.rows = N;
   walk.first = 0;
   walk.count = (kend + SR - 1) / SR;
-  // With a bias the nearest keys weigh most: a causal walk that starts at the
-  // diagonal finds the running maximum at once.  With ids, the diagonal tile is
-  // sure to be needed.
+  // With a bias the nearest keys weigh most: a walk that starts at the diagonal
+  // finds the running maximum at once (full [8,16,577,80] @I).  With ids, the
+  // diagonal tile is sure to be needed.
   walk.rev = p.causal && (bias || docs);
-  walk.own = docs && p.causal && pre == 0;
+  walk.start = !p.causal && (bias || docs) ? q0 / SR : 0;
+  walk.own = docs && pre == 0;
 
   Ring ring(smem, tid, D);
   auto fetch = [&](int tile, int, int stage) {
     if constexpr (DMA) ring.dma(kp, vp, nullptr, nullptr, tile * SR, N, D, stage);
     else ring.load(kp, vp, nullptr, nullptr, tile * SR, N, D);
+    if (docs) fetch_ids<SR, DMA>(walk.ids, tile * SR, N, s_ids[stage]);
   };
   // Every read that the walk waits for is issued here, before the first wait:
   // ids, this lane's rows, the first tile.
-  int my_id = 0, wlo = 0, whi = 0, block_id[RW * kRows / 64];
+  int my_id = 0, wlo = 0, whi = 0, block_id[(RW * kRows + 63) / 64];
   typename TileWalk<SPLIT>::Ids group_ids;
   if (docs) {
     walk.load(group_ids);
     my_id = qrow < N ? walk.ids[qrow] : -1;
 #pragma unroll
-    for (int i = 0; i < RW * kRows / 64; ++i) block_id[i] = q0 + lane + 64 * i < N ? walk.ids[q0 + lane + 64 * i] : -1;
+    for (int i = 0; i < (RW * kRows + 63) / 64; ++i) {
+      const int r = q0 + (lane + 64 * i) % (RW * kRows);
+      block_id[i] = r < N ? walk.ids[r] : -1;
+    }
   }
   // resident B operands: lane's query row, d = 16 kk + 8 hi .. +8
   F qf[KK], df[KK], of[KK];
@@ -445,7 +482,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
     whi = wave_max_i(my_id);
     int lo = 0x7fffffff, top = -1;
 #pragma unroll
-    for (int i = 0; i < RW * kRows / 64; ++i) {
+    for (int i = 0; i < (RW * kRows + 63) / 64; ++i) {
       lo = min(lo, block_id[i] < 0 ? 0x7fffffff : block_id[i]);
       top = max(top, block_id[i]);
     }
@@ -483,7 +520,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
   const float c = cap || bias ? 1.0f : p.scale_log2;
   const Reader<T, DP> rd(lane);
   constexpr unsigned kSubBytes = kRows * Layout<T, DP>::LD * sizeof(T);
-  stream_tiles<T, Ring, DMA, SPLIT>(ring, walk, 1, sub, N, fetch, [&](int stage, int tile, int, int id) {
+  stream_tiles<T, Ring, DMA, SPLIT>(ring, walk, 1, sub, s_ids, fetch, [&](int stage, int tile, int, int id) {
     const int kt = tile * SR + sub * kRows;
     if (kt >= kend_w) return;                               // past this wave's rows
     if (docs && id >= 0 && (id < wlo || id > whi)) return;  // a document of other waves' rows
@@ -504,12 +541,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
     float16_t dt;  // dQ: derivative of the cap
     if constexpr (MODE == 1) {
       if (cap) {
-        const float inv = 1.0f / p.cap_log2;
+        const float inv2 = -p.cap_slope;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float t = s[r] * inv;
-          dt[r] = fmaf(-t, t, 1.0f);
-        }
+        for (int r = 0; r < 16; ++r) dt[r] = fmaf(s[r] * s[r], inv2, 1.0f);
       }
     }
     if (bias) add_bias(s, slope2, static_cast<float>(kt + 4 * hi - qrow));
@@ -523,7 +557,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = my_id == id ? s[r] : -INFINITY;
       } else {
-        compare_ids(walk.ids, kt + 4 * hi, N, my_id, [&](int r, bool same) { s[r] = same ? s[r] : -INFINITY; });
+        compare_ids(s_ids[stage] + sub * kRows + 4 * hi, my_id, [&](int r, bool same) { s[r] = same ? s[r] : -INFINITY; });
       }
     }
     float16_t pm;  // P^T (forward) or dS^T (dQ)
@@ -638,10 +672,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int rr = 0; rr < 4; ++rr) {
-      const int d0 = 32 * db + 8 * rr + 4 * hi;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (ROWS == kRowFull || d0 + j < D) op[d0 + j] = static_cast<T>(live ? acc[db][4 * rr + j] * mul : 0.0f);
+      auto x = [&](int j) { return live ? acc[db][4 * rr + j] * mul : 0.0f; };
+      store4<T, ROWS>(op, 32 * db + 8 * rr + 4 * hi, D, x(0), x(1), x(2), x(3));
     }
 }
 
@@ -649,7 +681,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
 // Key-major kernel for 32 keys per wave: PASS 0 = dV, 1 = dK, 2 = both.
 constexpr int kPassDV = 0, kPassDK = 1, kPassBoth = 2;
 template <typename T, int DP, int DC, int ROWS, int PASS, int SPLIT, int MODS>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP <= 64 ? 2 : 1))) void scored_key_kernel(
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP <= 64 && SPLIT <= 2 ? 2 : 1))) void scored_key_kernel(
     ScoredParams p) {
   constexpr bool DO_DV = PASS != kPassDK;
   constexpr bool DO_DK = PASS != kPassDV;
@@ -660,6 +692,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
   constexpr int RW = kWaves / SPLIT;  // 32-key blocks per workgroup
   typedef TileRing<T, DP, DMA, true, kRows * SPLIT, ROWS> Ring;
   __shared__ __attribute__((aligned(1024))) char smem[Ring::BYTES];
+  __shared__ __attribute__((aligned(16))) int s_ids[2][kStagedIds];
 
   const int N = p.N, D = p.D;
   int u, hg, blk;
@@ -703,15 +736,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
     const float* second = DO_DK ? p.delta + head * N : lse;
     if constexpr (DMA) ring.dma(qp, dp, lse, second, qstart + tile * SR, N, D, stage);
     else ring.load(qp, dp, lse, second, qstart + tile * SR, N, D);
+    if (docs) fetch_ids<SR, DMA>(walk.ids, qstart + tile * SR, N, s_ids[stage]);
   };
   // every read that the walk waits for, before the first wait
-  int my_id = 0, wlo = 0, whi = 0, block_id[RW * kRows / 64];
+  int my_id = 0, wlo = 0, whi = 0, block_id[(RW * kRows + 63) / 64];
   typename TileWalk<SPLIT>::Ids group_ids;
   if (docs) {
     walk.load(group_ids);
     my_id = krow < N ? walk.ids[krow] : -1;
 #pragma unroll
-    for (int i = 0; i < RW * kRows / 64; ++i) block_id[i] = k0 + lane + 64 * i < N ? walk.ids[k0 + lane + 64 * i] : -1;
+    for (int i = 0; i < (RW * kRows + 63) / 64; ++i) {
+      const int r = k0 + (lane + 64 * i) % (RW * kRows);
+      block_id[i] = r < N ? walk.ids[r] : -1;
+    }
   }
   F kf[KK], vf[KK];
   {
@@ -729,7 +766,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
     whi = wave_max_i(my_id);
     int lo = 0x7fffffff, top = -1;
 #pragma unroll
-    for (int i = 0; i < RW * kRows / 64; ++i) {
+    for (int i = 0; i < (RW * kRows + 63) / 64; ++i) {
       lo = min(lo, block_id[i] < 0 ? 0x7fffffff : block_id[i]);
       top = max(top, block_id[i]);
     }
@@ -760,7 +797,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
 
   const Reader<T, DP> rd(lane);
   constexpr unsigned kSubBytes = kRows * Layout<T, DP>::LD * sizeof(T);
-  stream_tiles<T, Ring, DMA, SPLIT>(ring, walk, p.G, sub, N, fetch, [&](int stage, int tile, int g, int id) {
+  stream_tiles<T, Ring, DMA, SPLIT>(ring, walk, p.G, sub, s_ids, fetch, [&](int stage, int tile, int g, int id) {
     const int qt = qstart + tile * SR + sub * kRows;
     if (qt >= N || wk0 >= N) return;
     if (!every && wk0 >= pre && qt + kRows <= wk0) return;  // rows before every key of the wave
@@ -788,12 +825,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
     float16_t dt;
     if constexpr (DO_DK) {
       if (cap) {
-        const float inv = 1.0f / p.cap_log2;
+        const float inv2 = -p.cap_slope;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float t = s[r] * inv;
-          dt[r] = fmaf(-t, t, 1.0f);
-        }
+        for (int r = 0; r < 16; ++r) dt[r] = fmaf(s[r] * s[r], inv2, 1.0f);
       }
     }
     if (bias) add_bias(s, p.slopes[hk * p.G + g] * kLog2e, static_cast<float>(qt + 4 * hi - krow));
@@ -837,7 +871,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
 #pragma unroll
         for (int r = 0; r < 16; ++r) keep(r, my_id == id);
       } else {
-        compare_ids(walk.ids, qt + 4 * hi, N, my_id, keep);
+        compare_ids(s_ids[stage] + sub * kRows + 4 * hi, my_id, keep);
       }
     }
     if constexpr (DO_DV) {
@@ -896,12 +930,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
 #pragma unroll
     for (int rr = 0; rr < 4; ++rr) {
       const int d0 = 32 * db + 8 * rr + 4 * hi;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (ROWS == kRowFull || d0 + j < D) {
-          if constexpr (DO_DK) dkp[d0 + j] = static_cast<T>(dk[db][4 * rr + j] * p.scale);
-          if constexpr (DO_DV) dvp[d0 + j] = static_cast<T>(dv[db][4 * rr + j]);
-        }
+      auto x = [&](int j) { return dk[db][4 * rr + j] * p.scale; };
+      auto y = [&](int j) { return dv[db][4 * rr + j]; };
+      if constexpr (DO_DK) store4<T, ROWS>(dkp, d0, D, x(0), x(1), x(2), x(3));
+      if constexpr (DO_DV) store4<T, ROWS>(dvp, d0, D, y(0), y(1), y(2), y(3));
     }
 }
 

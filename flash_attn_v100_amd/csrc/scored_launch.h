@@ -36,46 +36,54 @@ inline long long deal_query(ScoredParams& p) {
   return deal(p, static_cast<long long>(p.B) * p.H_Q, 1);
 }
 
-template <typename T, int DP, int DC, int ROWS, int MODE, int MODS>
-void launch_query(ScoredParams p, bool split, hipStream_t st) {
-  if (ROWS != kRowElems && split) {
-    p.nblk = ceil_div(p.N, kBlockRows / 2);
-    const dim3 grid(static_cast<unsigned>(deal_query(p)));
-    hipLaunchKernelGGL((scored_query_kernel<T, DP, DC, ROWS, MODE, ROWS == kRowElems ? 1 : 2, MODS>), grid, dim3(kThreads), 0, st, p);
-    return;
+// Calls run(SPLIT) with the waves that share a row block as a compile-time number:
+// 1, 2, or 4 where four waves' tiles fit LDS (fp16 rows of at most 128, fp32 of 64).
+template <typename T, int DP, int ROWS, typename Run>
+void by_split(int split, Run&& run) {
+  if constexpr (ROWS != kRowElems) {
+    if constexpr (DP * sizeof(T) <= 256) {
+      if (split == 4) return run(std::integral_constant<int, 4>());
+    }
+    if (split >= 2) return run(std::integral_constant<int, 2>());
   }
-  p.nblk = ceil_div(p.N, kBlockRows);
-  const dim3 grid(static_cast<unsigned>(deal_query(p)));
-  hipLaunchKernelGGL((scored_query_kernel<T, DP, DC, ROWS, MODE, 1, MODS>), grid, dim3(kThreads), 0, st, p);
+  run(std::integral_constant<int, 1>());
+}
+
+template <typename T, int DP, int DC, int ROWS, int MODE, int MODS>
+void launch_query(ScoredParams p, int split, hipStream_t st) {
+  by_split<T, DP, ROWS>(split, [&](auto s) {
+    p.nblk = ceil_div(p.N, kBlockRows / s());
+    const dim3 grid(static_cast<unsigned>(deal_query(p)));
+    hipLaunchKernelGGL((scored_query_kernel<T, DP, DC, ROWS, MODE, s(), MODS>), grid, dim3(kThreads), 0, st, p);
+  });
 }
 
 template <typename T, int DP, int DC, int ROWS, int PASS, int MODS>
-void launch_key(ScoredParams p, bool split, hipStream_t st) {
-  const long long units = static_cast<long long>(p.B) * p.H_KV;
-  if (ROWS != kRowElems && split) {
-    p.nblk = ceil_div(p.N, kBlockRows / 2);
-    const dim3 grid(static_cast<unsigned>(deal(p, units, 1)));
-    hipLaunchKernelGGL((scored_key_kernel<T, DP, DC, ROWS, PASS, ROWS == kRowElems ? 1 : 2, MODS>), grid, dim3(kThreads), 0, st, p);
-    return;
-  }
-  p.nblk = ceil_div(p.N, kBlockRows);
-  const dim3 grid(static_cast<unsigned>(deal(p, units, 1)));
-  hipLaunchKernelGGL((scored_key_kernel<T, DP, DC, ROWS, PASS, 1, MODS>), grid, dim3(kThreads), 0, st, p);
+void launch_key(ScoredParams p, int split, hipStream_t st) {
+  by_split<T, DP, ROWS>(split, [&](auto s) {
+    p.nblk = ceil_div(p.N, kBlockRows / s());
+    const dim3 grid(static_cast<unsigned>(deal(p, static_cast<long long>(p.B) * p.H_KV, 1)));
+    hipLaunchKernelGGL((scored_key_kernel<T, DP, DC, ROWS, PASS, s(), MODS>), grid, dim3(kThreads), 0, st, p);
+  });
 }
 
-// Split blocks (two waves a block, half the walk each) where 128-row blocks
-// would leave CUs idle or with little to switch to.
-constexpr long long kSplitMaxBlocks = 512;
-inline bool split_query(const ScoredParams& p) {
-  return static_cast<long long>(p.B) * p.H_Q * ceil_div(p.N, kBlockRows) <= kSplitMaxBlocks;
+// Waves that share a row block (each walks 1 / split of its tiles), by the 128-row
+// blocks of the call: few blocks leave CUs idle or with little to switch to, and are
+// bound by the longest walk.
+inline int split_query(const ScoredParams& p, bool backward) {
+  const long long blocks = static_cast<long long>(p.B) * p.H_Q * ceil_div(p.N, kBlockRows);
+  if (blocks <= 64) return 4;
+  if (blocks <= 256) return 2;
+  return blocks <= 512 && (backward || (p.causal && p.N > 1024)) ? 2 : 1;
 }
-inline bool split_key(const ScoredParams& p) {
-  return static_cast<long long>(p.B) * p.H_KV * ceil_div(p.N, kBlockRows) <= kSplitMaxBlocks;
+inline int split_key(const ScoredParams& p) {
+  const long long blocks = static_cast<long long>(p.B) * p.H_KV * ceil_div(p.N, kBlockRows);
+  return blocks <= 64 ? 4 : (blocks <= 512 ? 2 : 1);
 }
 
 template <typename T, int DP, int DC, int ROWS, int MODS>
 void launch_backward_shape(const ScoredParams& p, hipStream_t st) {
-  launch_query<T, DP, DC, ROWS, 1, MODS>(p, split_query(p), st);
+  launch_query<T, DP, DC, ROWS, 1, MODS>(p, split_query(p, true), st);
   if constexpr (sizeof(T) == 2 && DP > 64) {
     launch_key<T, DP, DC, ROWS, kPassDV, MODS>(p, split_key(p), st);
     launch_key<T, DP, DC, ROWS, kPassDK, MODS>(p, split_key(p), st);

@@ -654,8 +654,8 @@ constexpr int kQuantum = kWaves * kTile;
 
 template <int CACHE>
 static int run(const char* fn, TokenParams p, float softcap, void* ws, size_t ws_bytes, hipStream_t st) {
-  if (softcap != 0.0f && !(softcap >= 1e-3f && softcap <= 1e6f))
-    return set_error(FA_ERR_INVALID_ARG, "%s: softcap must be 0 (none) or lie in [1e-3, 1e6]", fn);
+  if (softcap != 0.0f && !(softcap >= 1e-2f && softcap <= 1e3f))
+    return set_error(FA_ERR_INVALID_ARG, "%s: softcap must be 0 (none) or lie in [0.01, 1000]", fn);
   p.G = p.H_Q / p.H_KV;
   p.num_hg = ceil_div(p.G, kHeads);
   const float scale = 1.0f / sqrtf(static_cast<float>(p.D));

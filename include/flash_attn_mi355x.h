@@ -313,7 +313,7 @@ int fa_cross_gpu_allreduce_fp16(void* dst, const void* src, size_t n,
  * Self-attention with modified scores (no counterpart in the reference).
  *   q/o [B, H_Q, N, D], k/v [B, H_KV, N, D], H_Q % H_KV == 0; fp16: D <= 256,
  *   fp32: D <= 128.  lse fp32 [B, H_Q, N] or NULL (natural log).
- *   s = q.k / sqrt(D); softcap != 0 (in [1e-3, 1e6]): s = softcap * tanh(s / softcap);
+ *   s = q.k / sqrt(D); softcap != 0 (in [0.01, 1000]): s = softcap * tanh(s / softcap);
  *   slopes fp32 [H_Q] or NULL: s -= slopes[h] * |i - j|.
  *   Key j is visible to query i iff
  *     doc_ids == NULL or doc_ids[b, i] == doc_ids[b, j] >= 0  (int32 [B, N]), and
