@@ -752,7 +752,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> backward_scored(at::Tensor dout, 
   auto dv = at::empty_like(v);
   const int b = to_int(B, "B"), hq = to_int(H_Q, "H_Q"), hkv = to_int(k.size(1), "H_KV"), n = to_int(N, "N"),
             d = to_int(D, "D");
-  const size_t bytes = fa_backward_workspace_size(b, hq, n);
+  const size_t bytes = fa_scored_backward_workspace_size(b, hq, n);
   at::Tensor ws;
   if (bytes > 0) ws = at::empty({static_cast<int64_t>(bytes / sizeof(float))}, q.options().dtype(at::kFloat));
   auto fn = q.dtype() == at::kHalf ? fa_scored_backward_fp16 : fa_scored_backward_fp32;

@@ -76,7 +76,7 @@ static int backward(const char* fn, bool fp32, const void* dout, const void* q, 
   if (B == 0 || N == 0) return FA_OK;
   if (!dout || !q || !k || !v || !out || !lse || !dq || !dk || !dv)
     return set_error(FA_ERR_INVALID_ARG, "%s: null tensor pointer", fn);
-  const size_t need = fa_backward_workspace_size(B, H_Q, N);
+  const size_t need = fa_scored_backward_workspace_size(B, H_Q, N);
   if (!workspace || workspace_bytes < need)
     return set_error(FA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", fn, need,
                      workspace ? workspace_bytes : static_cast<size_t>(0));
@@ -84,6 +84,7 @@ static int backward(const char* fn, bool fp32, const void* dout, const void* q, 
   p.out = dq; p.dk = dk; p.dv = dv;
   p.lse = const_cast<float*>(lse);
   p.delta = static_cast<float*>(workspace);
+  p.row_lse = p.delta + static_cast<size_t>(B) * H_Q * N;
   const bool vec = aligned16(dout) && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(dq) &&
                    aligned16(dk) && aligned16(dv);
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -107,6 +108,11 @@ extern "C" int fa_scored_fp32(const void* q, const void* k, const void* v, void*
                               const int32_t* prefix_lens, void* stream) {
   return fa::scored::forward("fa_scored_fp32", true, q, k, v, o, lse, B, H_Q, H_KV, N, D, causal, softcap, slopes, doc_ids,
                              prefix_lens, stream);
+}
+
+extern "C" size_t fa_scored_backward_workspace_size(int B, int H_Q, int N) {
+  if (B <= 0 || H_Q <= 0 || N <= 0) return 0;
+  return 2 * static_cast<size_t>(B) * H_Q * N * sizeof(float);
 }
 
 extern "C" int fa_scored_backward_fp16(const void* dout, const void* q, const void* k, const void* v, const void* out,

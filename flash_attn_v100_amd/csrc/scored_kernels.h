@@ -67,7 +67,8 @@ struct ScoredParams {
   void* dk;
   void* dv;
   float* lse;             // forward: written if non-null; backward: read
-  float* delta;           // backward workspace [B * H_Q * N]
+  float* delta;           // backward workspace [B * H_Q * N]: delta, and
+  float* row_lse;         // [B * H_Q * N]: log-sum-exp as the key-major passes take it (dQ writes both)
   const float* slopes;    // [H_Q] or null
   const int32_t* ids;     // [B, N] or null
   const int32_t* prefix;  // [B] or null (causal only)
@@ -203,7 +204,7 @@ struct TileWalk {
   __device__ __forceinline__ void scan() {
     const int r0 = lane_row();
     masks([&](auto&& take) {
-#pragma unroll 2
+#pragma unroll 1
       for (int i = 0; i < kRows / 4; ++i) {
         const int4u x = *reinterpret_cast<const int4u*>(ids + r0 + 4 * i);
 #pragma unroll
@@ -254,6 +255,10 @@ struct TileWalk {
 };
 
 // ---- scores ----
+// A masked score of the backward: its P is 0, and its square stays finite in the
+// derivative of the cap.  Real ones lie far above (fp16 products within 1e12).
+constexpr float kDeadScore = -1e15f;
+
 // Raw products s -> capped scores in the log2 domain, cap log2(e) tanh(s scale / cap).
 // Where every score of the wave's tile is at most half the cap, tanh is the odd
 // polynomial of common.h with the scales folded into its coefficients, y = s (c0 +
@@ -312,6 +317,8 @@ __device__ __forceinline__ void compare_ids(const int* at, int mine, Use&& use) 
     const int4a x = *reinterpret_cast<const int4a*>(at + 8 * rr);
 #pragma unroll
     for (int j = 0; j < 4; ++j) use(4 * rr + j, max(x[j], -1) == mine);
+    // four ids at a time: the registers are full here, and such tiles are few
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
@@ -507,8 +514,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
 #pragma unroll
       for (int j = 0; j < 8; ++j) part = fmaf(static_cast<float>(df[kk][j]), static_cast<float>(of[kk][j]), part);
     delta = part + __shfl_xor(part, 32, 64);
-    if (qrow < N && hi == 0 && sub == 0) p.delta[qhead * N + qrow] = delta;
-    if (!live || lse2 == -INFINITY) lse2 = INFINITY;  // rows that see nothing: P = 0
+    const bool empty = !live || lse2 == -INFINITY;  // rows that see nothing: P = 0
+    if (qrow < N && hi == 0 && sub == 0) {
+      p.delta[qhead * N + qrow] = delta;
+      // the key-major passes mask scores to kDead, and so need a finite value (the
+      // register-staged ring scales by log2(e) itself)
+      p.row_lse[qhead * N + qrow] = empty ? 0.0f : (DMA ? lse2 : p.lse[qhead * N + qrow]);
+    }
+    if (empty) lse2 = INFINITY;
   }
 
   float16_t acc[DB];
@@ -538,26 +551,26 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] *= p.scale_log2;
     }
-    float16_t dt;  // dQ: derivative of the cap
-    if constexpr (MODE == 1) {
-      if (cap) {
-        const float inv2 = -p.cap_slope;
+    // dQ: derivative of the cap, from the capped score where that stays at hand
+    constexpr bool kKeepDt = MODE == 1 && (MODS & kAnyMods) != 0;
+    float16_t dt;
+    if constexpr (kKeepDt) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dt[r] = fmaf(s[r] * s[r], inv2, 1.0f);
-      }
+      for (int r = 0; r < 16; ++r) dt[r] = cap ? fmaf(s[r] * s[r], -p.cap_slope, 1.0f) : 1.0f;
     }
     if (bias) add_bias(s, slope2, static_cast<float>(kt + 4 * hi - qrow));
+    constexpr float kDead = MODE == 1 ? kDeadScore : -INFINITY;
     if (kt + kRows > N || (p.causal && kt + kRows - 1 > max(wq0, pre - 1))) {
       const int bound = last - kt - 4 * hi;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) > bound ? -INFINITY : s[r];
+      for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) > bound ? kDead : s[r];
     }
     if (docs && (id < 0 || id != wid)) {
       if (id >= 0) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = my_id == id ? s[r] : -INFINITY;
+        for (int r = 0; r < 16; ++r) s[r] = my_id == id ? s[r] : kDead;
       } else {
-        compare_ids(s_ids[stage] + sub * kRows + 4 * hi, my_id, [&](int r, bool same) { s[r] = same ? s[r] : -INFINITY; });
+        compare_ids(s_ids[stage] + sub * kRows + 4 * hi, my_id, [&](int r, bool same) { s[r] = same ? s[r] : kDead; });
       }
     }
     float16_t pm;  // P^T (forward) or dS^T (dQ)
@@ -601,10 +614,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) dp = mma(rd.row(vs, kk), df[kk], dp);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) pm[r] = fast_exp2(fmaf(s[r], c, -lse2)) * (dp[r] - delta);
-      if (cap) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) pm[r] *= dt[r];
+      for (int r = 0; r < 16; ++r) {
+        pm[r] = fast_exp2(fmaf(s[r], c, -lse2)) * (dp[r] - delta);
+        if constexpr (kKeepDt) pm[r] *= dt[r];
+        else if (cap) pm[r] *= fmaf(s[r] * s[r], -p.cap_slope, 1.0f);
       }
     }
     const F pf0 = acc_frag<T>(pm, 0), pf1 = acc_frag<T>(pm, 1);
@@ -681,7 +694,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
 // Key-major kernel for 32 keys per wave: PASS 0 = dV, 1 = dK, 2 = both.
 constexpr int kPassDV = 0, kPassDK = 1, kPassBoth = 2;
 template <typename T, int DP, int DC, int ROWS, int PASS, int SPLIT, int MODS>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP <= 64 && SPLIT <= 2 ? 2 : 1))) void scored_key_kernel(
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu((sizeof(T) == 4 ? DP <= 64 && SPLIT <= 2 : PASS == kPassBoth && DP == 128 && SPLIT <= 2 && (MODS & kAnyMods) == 0) ? 2 : 1))) void scored_key_kernel(
     ScoredParams p) {
   constexpr bool DO_DV = PASS != kPassDK;
   constexpr bool DO_DK = PASS != kPassDV;
@@ -731,7 +744,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
     const size_t head = qhead0 + g;
     const T* qp = static_cast<const T*>(p.q) + head * N * D;
     const T* dp = static_cast<const T*>(p.dout) + head * N * D;
-    const float* lse = p.lse + head * N;
+    const float* lse = p.row_lse + head * N;
     // the dV pass never reads delta: lse stands in for it in its stream
     const float* second = DO_DK ? p.delta + head * N : lse;
     if constexpr (DMA) ring.dma(qp, dp, lse, second, qstart + tile * SR, N, D, stage);
@@ -822,18 +835,32 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] *= p.scale_log2;
     }
+    // derivative of the cap: from the capped score where that is still at hand
+    constexpr bool kKeepDt = DO_DK && (MODS & kAnyMods) != 0;
     float16_t dt;
-    if constexpr (DO_DK) {
-      if (cap) {
-        const float inv2 = -p.cap_slope;
+    if constexpr (kKeepDt) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dt[r] = fmaf(s[r] * s[r], inv2, 1.0f);
-      }
+      for (int r = 0; r < 16; ++r) dt[r] = cap ? fmaf(s[r] * s[r], -p.cap_slope, 1.0f) : 1.0f;
     }
     if (bias) add_bias(s, p.slopes[hk * p.G + g] * kLog2e, static_cast<float>(qt + 4 * hi - krow));
+    if (qt + kRows > N || (!every && qt < wk0 + kRows - 1)) {
+      const int from = key_from - qt - 4 * hi, lim = N - qt - 4 * hi;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int rel = 8 * (r >> 2) + (r & 3);
+        s[r] = rel >= from && rel < lim ? s[r] : kDeadScore;
+      }
+    }
+    if (docs && (id < 0 || id != wid)) {
+      if (id >= 0) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = my_id == id ? s[r] : kDeadScore;
+      } else {
+        compare_ids(s_ids[stage] + sub * kRows + 4 * hi, my_id, [&](int r, bool same) { s[r] = same ? s[r] : kDeadScore; });
+      }
+    }
     const __attribute__((address_space(3))) float* lv = ring.vec(stage, 0) + sub * kRows;
     const __attribute__((address_space(3))) float* dvv = ring.vec(stage, 1) + sub * kRows;
-    const float lmul = DMA ? kLog2e : 1.0f;  // the register path stores lse pre-scaled
     float16_t pm, dsm;
 #pragma unroll
     for (int rr = 0; rr < 4; ++rr) {
@@ -843,35 +870,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = 4 * rr + j;
-        pm[r] = fast_exp2(fmaf(s[r], c, -l4[j] * lmul));
-        if constexpr (DO_DK) dsm[r] = (dp[r] - d4[j]) * pm[r];
-      }
-    }
-    if constexpr (DO_DK) {
-      if (cap) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dsm[r] *= dt[r];
-      }
-    }
-    // masks select, since a masked element may be infinite or NaN
-    auto keep = [&](int r, bool ok) {
-      pm[r] = ok ? pm[r] : 0.0f;
-      if constexpr (DO_DK) dsm[r] = ok ? dsm[r] : 0.0f;
-    };
-    if (qt + kRows > N || (!every && qt < wk0 + kRows - 1)) {
-      const int from = key_from - qt - 4 * hi, lim = N - qt - 4 * hi;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int rel = 8 * (r >> 2) + (r & 3);
-        keep(r, rel >= from && rel < lim);
-      }
-    }
-    if (docs && (id < 0 || id != wid)) {
-      if (id >= 0) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) keep(r, my_id == id);
-      } else {
-        compare_ids(s_ids[stage] + sub * kRows + 4 * hi, my_id, keep);
+        pm[r] = fast_exp2(fmaf(s[r], c, -l4[j]));
+        if constexpr (DO_DK) {
+          dsm[r] = (dp[r] - d4[j]) * pm[r];
+          if constexpr (kKeepDt) dsm[r] *= dt[r];
+          else if (cap) dsm[r] *= fmaf(s[r] * s[r], -p.cap_slope, 1.0f);
+        }
       }
     }
     if constexpr (DO_DV) {

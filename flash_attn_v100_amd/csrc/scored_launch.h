@@ -84,7 +84,7 @@ inline int split_key(const ScoredParams& p) {
 template <typename T, int DP, int DC, int ROWS, int MODS>
 void launch_backward_shape(const ScoredParams& p, hipStream_t st) {
   launch_query<T, DP, DC, ROWS, 1, MODS>(p, split_query(p, true), st);
-  if constexpr (sizeof(T) == 2 && DP > 64) {
+  if constexpr (sizeof(T) == 2 && DP > 64 && false) {
     launch_key<T, DP, DC, ROWS, kPassDV, MODS>(p, split_key(p), st);
     launch_key<T, DP, DC, ROWS, kPassDK, MODS>(p, split_key(p), st);
   } else {

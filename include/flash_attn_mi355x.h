@@ -336,9 +336,11 @@ int fa_scored_fp32(const void* q, const void* k, const void* v, void* o,
  * Its backward: dq [B, H_Q, N, D], dk/dv [B, H_KV, N, D] (summed over each KV
  * head's query heads, in a fixed order, without atomics) from dout, the
  * forward's inputs, its output and its lse.  D <= 128.  The workspace holds
- * fa_backward_workspace_size(B, H_Q, N) bytes and needs no initialisation.
+ * fa_scored_backward_workspace_size(B, H_Q, N) bytes (two fp32 a query row) and
+ * needs no initialisation.
  * softcap, slopes, doc_ids and prefix_lens are constants of the gradient.
  */
+size_t fa_scored_backward_workspace_size(int B, int H_Q, int N);
 int fa_scored_backward_fp16(const void* dout, const void* q, const void* k,
                             const void* v, const void* out, const float* lse,
                             void* dq, void* dk, void* dv, int B, int H_Q,
