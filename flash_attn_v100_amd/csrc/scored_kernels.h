@@ -77,6 +77,7 @@ struct ScoredParams {
   int nblk;               // row blocks (one workgroup each) per head
   int heads;              // query heads dealt with one unit (query-major)
   int units, group_units; // units of the grid, and how many an XCD interleaves
+  int snake;              // every other round of an XCD's blocks lightest first
   float scale;            // 1/sqrt(D)
   float scale_log2;       // scale * log2(e)
   float cap_in;           // scale / cap
@@ -93,11 +94,15 @@ __device__ __forceinline__ bool has(const ScoredParams& p, int m) {
 }
 
 constexpr int kXcds = 8;
+constexpr int kXcdCus = 32;
 
 // Workgroup -> (unit u, head of the unit, row block).  Units are dealt to the
 // XCDs round-robin (the dispatcher sends workgroup j to XCD j % 8), an XCD
 // interleaves group_units of them, heaviest block first, so the blocks that
-// stream the same tiles run together behind one L2.  Returns false for the
+// stream the same tiles run together behind one L2.  Heavy first suits grids
+// that the dispatcher refills as workgroups end; where the whole grid is
+// resident at once, workgroups i and i + 32 of an XCD share a CU, and the snake
+// order (every other 32 of them backwards) gives each CU about the same work.  Returns false for the
 // padding workgroups of the last round.  group_units 0: block by block, all
 // heads' heaviest first.
 __device__ __forceinline__ bool map_block(const ScoredParams& p, int heads, bool heavy_last, int& u, int& head, int& blk) {
@@ -111,8 +116,13 @@ __device__ __forceinline__ bool map_block(const ScoredParams& p, int heads, bool
   }
   const int i = j / kXcds;
   const int per_row = p.group_units * heads;
-  const int group = i / (per_row * p.nblk);
-  const int ii = i % (per_row * p.nblk);
+  const int n = per_row * p.nblk;
+  const int group = i / n;
+  int ii = i % n;
+  if (p.snake && ((ii / kXcdCus) & 1)) {
+    const int first = ii / kXcdCus * kXcdCus;
+    ii = first + min(n, first + kXcdCus) - 1 - ii;
+  }
   const int b = ii / per_row;
   const int hg = ii % per_row;
   u = j % kXcds + kXcds * (group * p.group_units + hg / heads);
