@@ -275,7 +275,7 @@ __host__ __device__ constexpr int long_chunk() { return MODE == kModePaged ? 768
 
 template <int MODE, int R>
 __device__ __forceinline__ RaggedItem ragged_item(const DecodeParams& p, int S) {
-  return ragged_item<R>([&](int q) { return seq_len_of<MODE>(p, q); }, p.B, p.H_KV * p.num_hg, p.plan_len, S,
+  return ragged_item<R>([&](int q) { return seq_len_of<MODE>(p, q); }, static_cast<int>(blockIdx.x), p.B, p.H_KV * p.num_hg, p.plan_len, S,
                         long_chunk<MODE>(), MODE == kModePaged);
 }
 

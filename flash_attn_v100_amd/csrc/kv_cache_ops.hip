@@ -4,7 +4,7 @@
 // ---- append (fa_paged_append_kv8) ----
 // A page of one head has one scale for its keys and one for its values:
 //   scale = max |x| (1 / top) over the page's tokens (top: 127 int8, 448 e4m3)
-//   code  = x / scale, clamped to +-top and rounded to nearest even
+//   code  = x / scale rounded to nearest even
 // A page that already holds tokens keeps the larger of its scale and the new
 // tokens' one; where it grows, the old codes are rounded again, code * old /
 // new.  All of it is IEEE fp32 arithmetic as written (1 / top rounded, one
@@ -23,6 +23,8 @@
 // row -> source token with one ballot scan, and a second kernel, with a
 // workgroup per 32 rows, copies the K and V rows of that map: the
 // part that is bound by bytes needs more workgroups than there are heads.
+#include <type_traits>
+
 #include "capi_internal.h"
 #include "common.h"
 
@@ -46,20 +48,44 @@ struct AppendParams {
   int pages_per_seq;  // pages a sequence's new tokens can touch
 };
 
-// x / scale as a code's value before rounding; 0 where the page is all zeros (a
-// NaN stays one).
-__device__ __forceinline__ float quotient(float x, float scale, float top) {
-  const float y = scale > 0.0f ? x / scale : 0.0f;
-  return y > top ? top : (y < -top ? -top : y);
-}
+// x / scale as a code's value before rounding, for one scale and many x: with r the
+// correctly rounded reciprocal, two residual corrections of x r give the correctly
+// rounded quotient (Markstein) in five operations where a division each takes twice as
+// many.  Nothing in between leaves fp32's normal numbers: fp16 x, and scales of their
+// maxima.  Scale 0 (a page of zeros) gives 0.  SIGNED: a zero keeps its sign, as a
+// quotient does (the corrections lose it; whole numbers have none).
+template <bool SIGNED>
+struct Divisor {
+  float scale, r;
+  uint32_t sign;
+  __device__ __forceinline__ explicit Divisor(float s)
+      : scale(s), r(s > 0.0f ? 1.0f / s : 0.0f), sign(s > 0.0f ? 0x80000000u : 0u) {}
+  __device__ __forceinline__ float operator()(float x) const {
+    float q = x * r;
+    q = fmaf(fmaf(-q, scale, x), r, q);
+    q = fmaf(fmaf(-q, scale, x), r, q);
+    if constexpr (!SIGNED) return q;
+    return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, q) | (__builtin_bit_cast(uint32_t, x) & sign));
+  }
+  // of a code that may be anything: clamped (a NaN stays one)
+  __device__ __forceinline__ float clamped(float x, float top) const {
+    const float y = (*this)(x);
+    return y > top ? top : (y < -top ? -top : y);
+  }
+};
+// Four quotients as codes.  Of values within the page's maximum none exceeds the
+// largest code by more than a rounding, which the rounding to a code takes back.
 template <bool FP8>
 __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
   if constexpr (FP8) {
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
     return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true));
   } else {
-    auto byte = [](float x) { return static_cast<uint32_t>(static_cast<int>(rintf(x))) & 0xffu; };
-    return byte(a) | byte(b) << 8 | byte(c) << 16 | byte(d) << 24;
+    // adding 1.5 2^23 rounds to nearest even and leaves the whole number in the low bits
+    auto bits = [](float x) { return __builtin_bit_cast(uint32_t, x + 12582912.0f); };
+    const uint32_t lo = __builtin_amdgcn_perm(bits(b), bits(a), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(bits(d), bits(c), 0x04000c0cu);
+    return lo | hi;
   }
 }
 // The values of 4 codes.
@@ -78,8 +104,9 @@ __device__ __forceinline__ void unpack4(uint32_t w, float (&x)[4]) {
   }
 }
 
-// VEC: D % 16 == 0, aligned rows: 16-value chunks; else single values.
-template <bool FP8, bool VEC>
+// VEC: D % 16 == 0, aligned rows: 16-value chunks, HOLD of them a lane kept in
+// registers; else single values.
+template <bool FP8, bool VEC, int HOLD = 1>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -100,7 +127,6 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
   const long long start = max(old, pi << p.page_shift), end = min(old + n, (pi + 1) << p.page_shift);
   if (start >= end || pi >= p.max_blocks) return;
   const int id = p.block_table[b * p.max_blocks + pi];
-  if (id < 0 || id >= p.num_pages) return;
 
   constexpr float kTop = FP8 ? 448.0f : 127.0f, kInvTop = 1.0f / kTop;
   const int D = p.D;
@@ -108,14 +134,9 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
   const int rows = static_cast<int>(end - start);
   const size_t stride = static_cast<size_t>(p.H_KV) * D;
   const half_t* src = (is_v ? p.v : p.k) + (from + static_cast<size_t>(start - old)) * stride + static_cast<size_t>(hkv) * D;
-  uint8_t* dst = (is_v ? p.v_cache : p.k_cache) + (((static_cast<size_t>(id) * p.H_KV + hkv) << p.page_shift)) * D;
-  float* scale_at = (is_v ? p.v_scale : p.k_scale) + static_cast<size_t>(id) * p.H_KV + hkv;
-  const float before = first > 0 ? *scale_at : 0.0f;
-
   if constexpr (VEC) {
     const int cpr = D / 16;
     const int chunks = rows * cpr;
-    constexpr int HOLD = 4;
     u32x4 held[HOLD][2];
     auto load = [&](int c, u32x4 (&x)[2]) {
       const half_t* at = src + static_cast<size_t>(c / cpr) * stride + c % cpr * 16;
@@ -134,6 +155,19 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
       held[i][0] = held[i][1] = u32x4{0u, 0u, 0u, 0u};
       if (lane + 64 * i < chunks) load(lane + 64 * i, held[i]);
     }
+    // the new rows are on their way while the page's id arrives; then its scale and
+    // old codes, which are needed only where the scale grows, together
+    if (id < 0 || id >= p.num_pages) return;
+    uint8_t* dst = (is_v ? p.v_cache : p.k_cache) + ((static_cast<size_t>(id) * p.H_KV + hkv) << p.page_shift) * D;
+    float* scale_at = (is_v ? p.v_scale : p.k_scale) + static_cast<size_t>(id) * p.H_KV + hkv;
+    const float before = first > 0 ? *scale_at : 0.0f;
+    const int old_chunks = first * cpr;
+    u32x4 old_codes[HOLD];
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i) {
+      old_codes[i] = u32x4{0u, 0u, 0u, 0u};
+      if (lane + 64 * i < old_chunks) old_codes[i] = *reinterpret_cast<const u32x4*>(dst + static_cast<size_t>(lane + 64 * i) * 16);
+    }
 #pragma unroll
     for (int i = 0; i < HOLD; ++i) raise(held[i]);
     for (int c = lane + 64 * HOLD; c < chunks; c += 64) {
@@ -143,6 +177,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
     }
     const float amax = wave_max(fmaxf(static_cast<float>(top2[0]), static_cast<float>(top2[1])));
     const float scale = fmaxf(amax * kInvTop, before);
+    const Divisor<FP8> by(scale);
     auto store = [&](int c, const u32x4 (&x)[2]) {
       u32x4 codes;
 #pragma unroll
@@ -151,7 +186,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const half2_t h = as_h2(x[q >> 1][2 * (q & 1) + (e >> 1)]);
-          y[e] = quotient(static_cast<float>(h[e & 1]), scale, kTop);
+          y[e] = by(static_cast<float>(h[e & 1]));
         }
         codes[q] = pack4<FP8>(y[0], y[1], y[2], y[3]);
       }
@@ -166,36 +201,43 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
       store(c, x);
     }
     if (first > 0 && scale > before) {
-      for (int c = lane; c < first * cpr; c += 64) {
-        u32x4* at = reinterpret_cast<u32x4*>(dst + static_cast<size_t>(c) * 16);
-        u32x4 codes = *at;
+      auto again = [&](int c, u32x4 codes) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           float y[4];
           unpack4<FP8>(codes[q], y);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = quotient(y[e] * before, scale, kTop);
+          for (int e = 0; e < 4; ++e) y[e] = by.clamped(y[e] * before, kTop);
           codes[q] = pack4<FP8>(y[0], y[1], y[2], y[3]);
         }
-        *at = codes;
-      }
+        *reinterpret_cast<u32x4*>(dst + static_cast<size_t>(c) * 16) = codes;
+      };
+#pragma unroll
+      for (int i = 0; i < HOLD; ++i)
+        if (lane + 64 * i < old_chunks) again(lane + 64 * i, old_codes[i]);
+      for (int c = lane + 64 * HOLD; c < old_chunks; c += 64) again(c, *reinterpret_cast<const u32x4*>(dst + static_cast<size_t>(c) * 16));
     }
     if (lane == 0) *scale_at = scale;
   } else {
+    if (id < 0 || id >= p.num_pages) return;
+    uint8_t* dst = (is_v ? p.v_cache : p.k_cache) + ((static_cast<size_t>(id) * p.H_KV + hkv) << p.page_shift) * D;
+    float* scale_at = (is_v ? p.v_scale : p.k_scale) + static_cast<size_t>(id) * p.H_KV + hkv;
+    const float before = first > 0 ? *scale_at : 0.0f;
     const int values = rows * D;
     float amax = 0.0f;
     for (int e = lane; e < values; e += 64) amax = fmaxf(amax, fabsf(static_cast<float>(src[static_cast<size_t>(e / D) * stride + e % D])));
     amax = wave_max(amax);
     const float scale = fmaxf(amax * kInvTop, before);
+    const Divisor<FP8> by(scale);
     for (int e = lane; e < values; e += 64) {
-      const float y = quotient(static_cast<float>(src[static_cast<size_t>(e / D) * stride + e % D]), scale, kTop);
+      const float y = by(static_cast<float>(src[static_cast<size_t>(e / D) * stride + e % D]));
       dst[static_cast<size_t>(first) * D + e] = static_cast<uint8_t>(pack4<FP8>(y, 0.0f, 0.0f, 0.0f));
     }
     if (first > 0 && scale > before) {
       for (int e = lane; e < first * D; e += 64) {
         float y[4];
         unpack4<FP8>(dst[e], y);
-        dst[e] = static_cast<uint8_t>(pack4<FP8>(quotient(y[0] * before, scale, kTop), 0.0f, 0.0f, 0.0f));
+        dst[e] = static_cast<uint8_t>(pack4<FP8>(by.clamped(y[0] * before, kTop), 0.0f, 0.0f, 0.0f));
       }
     }
     if (lane == 0) *scale_at = scale;
@@ -230,7 +272,7 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
 
 __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
   __shared__ int hist[kBins];
-  __shared__ int s_wave[2][kSelWaves];
+  __shared__ int s_wave[1][kSelWaves];
   __shared__ int s_pick[2];
   const int bh = blockIdx.x;
   const int b = bh / p.H_KV;
@@ -259,17 +301,34 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
   if (need == 0) return;
 
   // ---- the need-th largest key: digit by digit from the top ----
+  // Up to 8192 competing tokens' keys stay in registers, eight a thread; of longer
+  // caches they are read again for each digit.
+  constexpr int HELD = 8;
+  const bool held = head <= HELD * kSelThreads;
+  uint32_t keys[HELD];
+  if (held) {
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      const int t = tid + i * kSelThreads;
+      keys[i] = t < head ? weight_key(weight[t]) : 0u;
+    }
+  }
   uint32_t prefix = 0u, mask = 0u;
   int want = need;  // rank still sought among the keys that share the prefix
   constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const uint32_t digits = (1u << kBits[pass]) - 1u;
-    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+    hist[tid] = hist[tid + kSelThreads] = 0;
     __syncthreads();
-    for (int t = tid; t < head; t += kSelThreads) {
-      const uint32_t key = weight_key(weight[t]);
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> kShift[pass]) & digits], 1);
+    auto count = [&](int t, uint32_t key) {
+      if (t < head && (key & mask) == prefix) atomicAdd(&hist[(key >> kShift[pass]) & digits], 1);
+    };
+    if (held) {
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) count(tid + i * kSelThreads, keys[i]);
+    } else {
+      for (int t = tid; t < head; t += kSelThreads) count(t, weight_key(weight[t]));
     }
     __syncthreads();
     // thread t owns the bins 2t', 2t'+1 from the top
@@ -279,7 +338,8 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
     if (lane == 63) s_wave[0][wave] = incl;
     __syncthreads();
     int above = incl - c0 - c1;
-    for (int q = 0; q < wave; ++q) above += s_wave[0][q];
+#pragma unroll
+    for (int q = 0; q < kSelWaves; ++q) above += q < wave ? s_wave[0][q] : 0;
     if (above < want && above + c0 + c1 >= want) {  // exactly one thread
       const bool first = above + c0 >= want;
       s_pick[0] = first ? hi : hi - 1;
@@ -289,25 +349,29 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
     prefix |= static_cast<uint32_t>(s_pick[0]) << kShift[pass];
     mask |= digits << kShift[pass];
     want -= s_pick[1];
-    __syncthreads();
   }
 
   // ---- keys above the threshold stay, and the first `want` that equal it ----
   int gt_before = 0, eq_before = 0;
-  for (int base = 0; base < head; base += kSelThreads) {
+  int parity = 0;  // counts of alternate rounds lie apart: one barrier a round
+  __shared__ int s_count[2][2][kSelWaves];
+  float next = tid < head ? weight[tid] : 0.0f;
+  for (int base = 0; base < head; base += kSelThreads, parity ^= 1) {
     const int t = base + tid;
-    const float x = t < head ? weight[t] : 0.0f;
+    const float x = next;
+    if (t + kSelThreads < head) next = weight[t + kSelThreads];
     const uint32_t key = weight_key(x);
     const bool gt = t < head && key > prefix, eq = t < head && key == prefix;
     const uint64_t gts = __builtin_amdgcn_ballot_w64(gt), eqs = __builtin_amdgcn_ballot_w64(eq);
     if (lane == 0) {
-      s_wave[0][wave] = __builtin_popcountll(gts);
-      s_wave[1][wave] = __builtin_popcountll(eqs);
+      s_count[parity][0][wave] = __builtin_popcountll(gts);
+      s_count[parity][1][wave] = __builtin_popcountll(eqs);
     }
     __syncthreads();
     int g0 = gt_before, e0 = eq_before;
+#pragma unroll
     for (int q = 0; q < kSelWaves; ++q) {
-      const int g = s_wave[0][q], e = s_wave[1][q];
+      const int g = s_count[parity][0][q], e = s_count[parity][1][q];
       g0 += q < wave ? g : 0;
       e0 += q < wave ? e : 0;
       gt_before += g;
@@ -317,7 +381,6 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
     g0 += __builtin_popcountll(gts & below);
     e0 += __builtin_popcountll(eqs & below);
     if (gt || (eq && e0 < want)) emit(g0 + min(e0, want), t, x);
-    __syncthreads();
   }
 }
 
@@ -409,13 +472,17 @@ extern "C" int fa_paged_append_kv8(const void* k, const void* v, const int32_t* 
   const bool vec = D % 16 == 0 && aligned16(k) && aligned16(v) && aligned16(k_cache) && aligned16(v_cache);
   const dim3 grid(static_cast<unsigned>(blocks)), block(kvops::kThreads);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (fp8) {
-    if (vec) hipLaunchKernelGGL((kvops::append_kernel<true, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((kvops::append_kernel<true, false>), grid, block, 0, st, p);
-  } else {
-    if (vec) hipLaunchKernelGGL((kvops::append_kernel<false, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((kvops::append_kernel<false, false>), grid, block, 0, st, p);
-  }
+  // a page's chunks in registers: two a lane (16 tokens at D = 128) or four, past that
+  // the rest is read again
+  const bool two = page * D <= 2 * 64 * 16;
+  auto launch = [&](auto f8) {
+    constexpr bool F = decltype(f8)::value;
+    if (!vec) hipLaunchKernelGGL((kvops::append_kernel<F, false>), grid, block, 0, st, p);
+    else if (two) hipLaunchKernelGGL((kvops::append_kernel<F, true, 2>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((kvops::append_kernel<F, true, 4>), grid, block, 0, st, p);
+  };
+  if (fp8) launch(std::true_type());
+  else launch(std::false_type());
   return check_launch(fn);
 }
 

@@ -57,12 +57,12 @@ __device__ __forceinline__ int div_by(int a, int c, float inv) {
   return q + (r >= c ? 1 : 0) - (r < 0 ? 1 : 0);
 }
 
-// R: lengths a lane holds (B <= 64 R); len_of(q): keys of sequence q; per_seq:
+// item: which share (the workgroup's number); R: lengths a lane holds (B <= 64 R); len_of(q): keys of sequence q; per_seq:
 // units per sequence; plan_len: longest plannable sequence; S: splits a
 // sequence has room for; long_chunk: keys past which one round leaves the CUs
 // unevenly loaded; unsplit: enough sequences run unsplit.
 template <int R, typename LenOf>
-__device__ __forceinline__ RaggedItem ragged_item(LenOf&& len_of, int B, int per_seq, int plan_len, int S, int long_chunk,
+__device__ __forceinline__ RaggedItem ragged_item(LenOf&& len_of, int item, int B, int per_seq, int plan_len, int S, int long_chunk,
                                                   bool unsplit) {
   const int lane = threadIdx.x & 63;
   int len[R], plan[R], full[R], upto[R];
@@ -108,7 +108,6 @@ __device__ __forceinline__ RaggedItem ragged_item(LenOf&& len_of, int B, int per
     upto[i] = all + wave_scan_add(full[i]);
     all = __builtin_amdgcn_readlane(upto[i], 63);
   }
-  const int item = static_cast<int>(blockIdx.x);
   it.b = -1;
   it.unit = it.split = it.splits = it.len = 0;
   uint64_t in = 0;      // the lanes that may hold the item's sequence, in block `base` / 64,

@@ -62,7 +62,10 @@ constexpr unsigned kCounterSlots = 65536;  // arrival counters at the start of t
 constexpr int kMaxSplits = 128;
 constexpr int kPlanMaxSeqs = 512;
 constexpr int kStaticMaxBlocks = 600;
-constexpr int kLongChunk = 1280;
+// Ragged plans (ragged_plan.h): chunks past which one round leaves the CUs unevenly
+// loaded; enough sequences on the 8-bit cache run unsplit ([128] to 4096 of 32:8 heads
+// 103 us, split in 1280 106).
+constexpr int kLongChunk = 768;
 
 struct TokenParams {
   const half_t* q;
@@ -138,8 +141,23 @@ __device__ __forceinline__ half8_t codes8(u32x2 raw) {
   return half8_t{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
 }
 
+// Every argument at once: left to itself the compiler fetches them in dependent
+// rounds behind the early exits, a memory round trip each.
+template <int CACHE>
+__device__ __forceinline__ void preload_args(const TokenParams& p) {
+  asm volatile("" ::"s"(p.q), "s"(p.k), "s"(p.v), "s"(p.o), "s"(p.lens), "s"(p.slopes), "s"(p.scores), "s"(p.lse));
+  asm volatile("" ::"s"(p.ws_o), "s"(p.ws_lse), "s"(p.counters), "s"(p.unit_base), "s"(p.len_plus), "s"(p.cap_in), "s"(p.cap_log2));
+  asm volatile("" ::"s"(p.B), "s"(p.H_Q), "s"(p.H_KV), "s"(p.N), "s"(p.D), "s"(p.G), "s"(p.num_hg), "s"(p.chunk));
+  asm volatile("" ::"s"(p.num_splits), "s"(p.ragged), "s"(p.scale_log2));
+  if constexpr (CACHE != kF16)
+    asm volatile("" ::"s"(p.k_scale), "s"(p.v_scale), "s"(p.block_table), "s"(p.max_blocks), "s"(p.num_pages), "s"(p.page_shift));
+}
+
+// Registers: 8-bit rows of up to 128 leave room for four waves per SIMD (their tiles
+// are half as large: LDS holds four workgroups).
 template <int DP, int ROWS, int CACHE>
-__global__ __launch_bounds__(kThreads) void token_kernel(TokenParams p) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(CACHE != kF16 && DP <= 128 && ROWS != kRowElems ? 4 : 1))) void token_kernel(
+    TokenParams p) {
   constexpr bool C8 = CACHE != kF16;
   constexpr int ES = C8 ? 1 : 2;
   constexpr int RB = DP * ES;               // LDS row bytes
@@ -157,6 +175,7 @@ __global__ __launch_bounds__(kThreads) void token_kernel(TokenParams p) {
   __shared__ float s_m[kWaves][kHeads], s_l[kWaves][kHeads];
   __shared__ int s_bad, s_last;
 
+  preload_args<CACHE>(p);
   const int S = p.num_splits, D = p.D, G = p.G;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -168,10 +187,15 @@ __global__ __launch_bounds__(kThreads) void token_kernel(TokenParams p) {
   if (p.ragged) {
     auto len = [&](int b) { return len_of(p, b); };
     const int per_seq = p.H_KV * p.num_hg;
-    const RaggedItem it = p.B <= 64    ? ragged_item<1>(len, p.B, per_seq, p.N, S, kLongChunk, false)
-                          : p.B <= 128 ? ragged_item<2>(len, p.B, per_seq, p.N, S, kLongChunk, false)
-                          : p.B <= 256 ? ragged_item<4>(len, p.B, per_seq, p.N, S, kLongChunk, false)
-                                       : ragged_item<kPlanMaxSeqs / 64>(len, p.B, per_seq, p.N, S, kLongChunk, false);
+    // A page's scales lie side by side for all its heads, one line for the units of a
+    // sequence: workgroups go to XCD j % 8, and within every whole 64 of them an XCD takes
+    // eight neighbours, so that eight heads share a line in one L2 (@J).
+    int item = static_cast<int>(blockIdx.x);
+    if (C8 && (item | 63) < static_cast<int>(gridDim.x)) item = (item & ~63) | (item & 7) << 3 | (item >> 3 & 7);
+    const RaggedItem it = p.B <= 64    ? ragged_item<1>(len, item, p.B, per_seq, p.N, S, kLongChunk, C8)
+                          : p.B <= 128 ? ragged_item<2>(len, item, p.B, per_seq, p.N, S, kLongChunk, C8)
+                          : p.B <= 256 ? ragged_item<4>(len, item, p.B, per_seq, p.N, S, kLongChunk, C8)
+                                       : ragged_item<kPlanMaxSeqs / 64>(len, item, p.B, per_seq, p.N, S, kLongChunk, C8);
     if (it.b < 0) return;
     chunk = it.chunk;
     split = it.split;
@@ -217,17 +241,23 @@ __global__ __launch_bounds__(kThreads) void token_kernel(TokenParams p) {
         id = 0;
       }
       s_page[i] = id;
-      const size_t at = static_cast<size_t>(id) * p.H_KV + hkv;
+    }
+    round = from;
+  };
+  // Their scales, read while the first tiles travel.
+  auto stage_scales = [&](int from, int to) {
+    const int np = ((to - 1) >> p.page_shift) - (from >> p.page_shift) + 1;
+    for (int i = tid; i < np; i += kThreads) {
+      const size_t at = static_cast<size_t>(s_page[i]) * p.H_KV + hkv;
       s_ks[i] = p.k_scale[at];
       s_vs[i] = p.v_scale[at];
     }
-    __syncthreads();
-    round = from;
   };
   if constexpr (C8) {
     if (tid == 0) s_bad = too_long ? 1 : 0;
     __syncthreads();
     stage_pages(k0, min(k1, k0 + kRoundKeys));
+    __syncthreads();
   }
   auto slot_of = [&](int t) { return (t >> p.page_shift) - (round >> p.page_shift); };
 
@@ -323,6 +353,10 @@ __global__ __launch_bounds__(kThreads) void token_kernel(TokenParams p) {
   auto walk = [&](int from, int to) __attribute__((always_inline)) {
     int t0 = from + wave * kTile;
     if (t0 < to) issue(t0);
+    if constexpr (C8) {
+      stage_scales(from, to);
+      __syncthreads();
+    }
     while (t0 < to) {
       wait_vm_lgkm0<0>();  // the tile has landed (the copies are this wave's own)
       __builtin_amdgcn_wave_barrier();
@@ -468,6 +502,7 @@ __global__ __launch_bounds__(kThreads) void token_kernel(TokenParams p) {
       if (rb != k0) {
         __syncthreads();  // every wave is done with the previous round's ids
         stage_pages(rb, re);
+        __syncthreads();
       }
       walk(rb, re);
     }
@@ -539,7 +574,7 @@ __global__ __launch_bounds__(kThreads) void token_kernel(TokenParams p) {
   // columns of 4 outputs over the threads, spare threads taking splits in phases
   const int ncol = g_valid * NC4;
   const int phases = ncol >= kThreads ? 1 : kThreads / ncol;
-  constexpr int BATCH = 8;
+  constexpr int BATCH = C8 ? 8 : 20;  // loads in flight: a phase of a 33-split merge waits once
   float4_t* s_num = reinterpret_cast<float4_t*>(smem);                       // [kThreads]
   float* s_den = reinterpret_cast<float*>(smem) + 4 * kThreads;              // [kThreads]
   float* s_max = s_den + kThreads;                                           // [kThreads]
@@ -610,18 +645,33 @@ __global__ __launch_bounds__(kThreads) void token_kernel(TokenParams p) {
 
 // weight_out[b, h_kv, t] = weight[b, h_kv, t] + sum over the KV head's query
 // heads of exp2(score - lse), for the keys of each sequence; other entries are
-// left as they are.  One thread per key, a head's rows read in turn.
+// left as they are.  VEC: four keys a thread (N % 4 == 0, aligned arrays).
+template <bool VEC>
 __global__ __launch_bounds__(kThreads) void add_weights_kernel(TokenParams p, const float* weight, float* weight_out) {
+  constexpr int K = VEC ? 4 : 1;
+  typedef float vec __attribute__((ext_vector_type(K)));
   const int pair = blockIdx.y;
   const int b = pair / p.H_KV, hkv = pair % p.H_KV;
   const int L = len_of(p, b);
-  const int t = static_cast<int>(blockIdx.x) * kThreads + threadIdx.x;
+  const int t = (static_cast<int>(blockIdx.x) * kThreads + threadIdx.x) * K;
   if (t >= L) return;
   const size_t bh = static_cast<size_t>(b) * p.H_Q + hkv * p.G;
   const size_t at = static_cast<size_t>(pair) * p.N + t;
-  float sum = weight[at];
-  for (int g = 0; g < p.G; ++g) sum += fast_exp2(p.scores[(bh + g) * p.N + t] - p.lse[bh + g]);
-  weight_out[at] = sum;
+  vec sum = *reinterpret_cast<const vec*>(weight + at);
+  for (int g = 0; g < p.G; ++g) {
+    // (scores past the last key were never written: what comes of them is not stored)
+    const vec s = *reinterpret_cast<const vec*>(p.scores + (bh + g) * p.N + t);
+    const float lse = p.lse[bh + g];
+#pragma unroll
+    for (int j = 0; j < K; ++j) sum[j] += fast_exp2(s[j] - lse);
+  }
+  if (t + K <= L) {
+    *reinterpret_cast<vec*>(weight_out + at) = sum;
+  } else {
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+      if (t + j < L) weight_out[at + j] = sum[j];
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -645,12 +695,22 @@ static void dispatch(int dp, int rows, const TokenParams& p, int blocks, hipStre
   else by_rows(w256);
 }
 
-// Splits: chunks of a multiple of 128 keys (one tile a wave) for about
-// kTargetBlocks workgroups, at most kMaxChunk keys and kMaxSplits of them.
+// Splits of equal chunks for about `target` workgroups: chunks of a multiple of 128
+// keys (one tile a wave), at most kMaxChunk keys and kMaxSplits of them.
 // fa_decode_workspace_size covers it: its bound takes the same quantum and a
-// larger target.
-constexpr int kTargetBlocks = 1024;
+// target of kRaggedTarget.
+constexpr int kStaticTarget = 1024;
+constexpr int kRaggedTarget = 4096;
 constexpr int kQuantum = kWaves * kTile;
+
+struct Splits {
+  long long chunk, count;
+};
+static Splits plan_splits(long long len, long long units, int target) {
+  long long chunk = std::max((len * units + target - 1) / target, (len + kMaxSplits - 1) / kMaxSplits);
+  chunk = std::min<long long>((chunk + kQuantum - 1) / kQuantum * kQuantum, kMaxChunk);
+  return {chunk, (len + chunk - 1) / chunk};
+}
 
 template <int CACHE>
 static int run(const char* fn, TokenParams p, float softcap, void* ws, size_t ws_bytes, hipStream_t st) {
@@ -665,13 +725,15 @@ static int run(const char* fn, TokenParams p, float softcap, void* ws, size_t ws
   const int dp = p.D <= 64 ? 64 : (p.D <= 128 ? 128 : 256);
   const long long units = static_cast<long long>(p.B) * p.H_KV * p.num_hg;
   const long long len = std::max(p.N, 1);
-  long long chunk = (len * units + kTargetBlocks - 1) / kTargetBlocks;
-  chunk = std::max(chunk, (len + kMaxSplits - 1) / kMaxSplits);
-  chunk = std::min<long long>((chunk + kQuantum - 1) / kQuantum * kQuantum, kMaxChunk);
-  const long long splits = (len + chunk - 1) / chunk;
+  Splits plan = plan_splits(len, units, kStaticTarget);
+  // more work than is resident at once: planned from the lengths on the device,
+  // with room for shorter splits
+  const bool many = units * plan.count > kStaticMaxBlocks && p.B <= kPlanMaxSeqs && units <= static_cast<long long>(kCounterSlots);
+  if (many) plan = plan_splits(len, units, kRaggedTarget);
+  const long long splits = plan.count;
   if (splits > kMaxSplits)
     return set_error(FA_ERR_UNSUPPORTED, "%s: %d keys per sequence exceed %d", fn, p.N, kMaxSplits * kMaxChunk);
-  p.chunk = static_cast<int>(chunk);
+  p.chunk = static_cast<int>(plan.chunk);
   p.num_splits = static_cast<int>(splits);
   if (splits > 1) {
     const size_t entries = static_cast<size_t>(p.B) * p.H_Q * splits;
@@ -690,7 +752,7 @@ static int run(const char* fn, TokenParams p, float softcap, void* ws, size_t ws
   const int per_chunk = CACHE == kF16 ? 8 : 16;
   const bool vec = aligned16(p.q) && aligned16(p.k) && aligned16(p.v) && p.D % per_chunk == 0;
   const int rows = !vec ? kRowElems : (p.D == dp ? kRowFull : kRowChunks);
-  if (splits > 1 && units * splits > kStaticMaxBlocks && p.B <= kPlanMaxSeqs && units <= static_cast<long long>(kCounterSlots)) {
+  if (many && splits > 1) {
     const long long full = std::max<long long>(kRoundBlocks, std::min<long long>(kManyBlocks, units * len / kLongChunk));
     p.ragged = 1;
     dispatch<CACHE>(dp, rows, p, static_cast<int>(full + units), st);
@@ -721,6 +783,8 @@ static int contiguous(const char* fn, const void* q, const void* k, const void* 
   if (const int rc = check_sizes(fn, B, H_Q, H_KV, D)) return rc;
   if (N <= 0) return set_error(FA_ERR_INVALID_ARG, "%s: N must be positive", fn);
   if (B > 0 && (!q || !k || !v || !o || !cache_lens)) return set_error(FA_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (weighted && (reinterpret_cast<uintptr_t>(scores) & 15) != 0)
+    return set_error(FA_ERR_INVALID_ARG, "%s: scratch must be 16-byte aligned", fn);
   if (B > 0 && weighted && (!weight || !weight_out || !scores)) return set_error(FA_ERR_INVALID_ARG, "%s: null pointer", fn);
   if (weighted && static_cast<long long>(B) * H_KV > 65535)
     return set_error(FA_ERR_UNSUPPORTED, "%s: more than 65535 (sequence, KV head) pairs", fn);
@@ -741,7 +805,10 @@ static int contiguous(const char* fn, const void* q, const void* k, const void* 
   const int rc = run<kF16>(fn, p, softcap, ws, ws_bytes, st);
   if (rc != FA_OK || !weighted || B == 0) return rc;
   p.G = H_Q / H_KV;
-  hipLaunchKernelGGL(add_weights_kernel, dim3(ceil_div(N, kThreads), B * H_KV), dim3(kThreads), 0, st, p, weight, weight_out);
+  const bool vec = N % 4 == 0 && aligned16(weight) && aligned16(weight_out) && aligned16(scores);
+  const dim3 grid(ceil_div(N, kThreads * (vec ? 4 : 1)), B * H_KV);
+  if (vec) hipLaunchKernelGGL(add_weights_kernel<true>, grid, dim3(kThreads), 0, st, p, weight, weight_out);
+  else hipLaunchKernelGGL(add_weights_kernel<false>, grid, dim3(kThreads), 0, st, p, weight, weight_out);
   return check_launch(fn);
 }
 

@@ -375,7 +375,8 @@ int fa_decode_scored_fp16(const void* q, const void* k, const void* v, void* o,
  *   heads of their softmax weight of key t, for the keys attended; other
  *   entries of weight_out are left as they are.  weight/weight_out fp32 [B,
  *   H_KV, N]; they may be one array.  The scratch holds
- *   fa_decode_weighted_scratch_size(B, H_Q, N) bytes and needs no initialisation.
+ *   fa_decode_weighted_scratch_size(B, H_Q, N) bytes, 16-byte aligned, and needs no
+ *   initialisation.
  *   B * H_KV <= 65535.  Two launches.
  */
 size_t fa_decode_weighted_scratch_size(int B, int H_Q, int N);
