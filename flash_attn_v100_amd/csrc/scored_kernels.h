@@ -275,16 +275,20 @@ constexpr float kDeadScore = -1e15f;
 // c1 s^2 + ...): 6 full-rate operations a score, where the exponential form takes two
 // quarter-rate ones and 9 others.  (These kernels are bound by their vector
 // instructions: with the coefficients unfolded, 9 a score, @E.)
-__device__ __forceinline__ void cap_scores(float16_t& s, const ScoredParams& p) {
+__device__ __forceinline__ float cap_factor(float s, const ScoredParams& p) {
+  const float w = s * s;
+  return fmaf(fmaf(fmaf(fmaf(p.cap_poly[4], w, p.cap_poly[3]), w, p.cap_poly[2]), w, p.cap_poly[1]), w, p.cap_poly[0]);
+}
+__device__ __forceinline__ bool cap_is_near(const float16_t& s, const ScoredParams& p) {
   float big = 0.0f;
 #pragma unroll
   for (int r = 0; r < 16; r += 2) big = fmaxf(fmaxf(fabsf(s[r]), fabsf(s[r + 1])), big);
-  if (__builtin_amdgcn_ballot_w64(!(big <= p.cap_near)) == 0) {
+  return __builtin_amdgcn_ballot_w64(!(big <= p.cap_near)) == 0;
+}
+__device__ __forceinline__ void cap_scores(float16_t& s, bool near, const ScoredParams& p) {
+  if (near) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float w = s[r] * s[r];
-      s[r] *= fmaf(fmaf(fmaf(fmaf(p.cap_poly[4], w, p.cap_poly[3]), w, p.cap_poly[2]), w, p.cap_poly[1]), w, p.cap_poly[0]);
-    }
+    for (int r = 0; r < 16; ++r) s[r] *= cap_factor(s[r], p);
   } else {
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = tanh_f32(s[r] * p.cap_in) * p.cap_log2;
@@ -555,9 +559,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
     for (int r = 0; r < 16; ++r) s[r] = 0.0f;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) s = mma(rd.row(ks, kk), qf[kk], s);
-    if (cap) {
-      cap_scores(s, p);
-    } else if (bias) {
+    const bool edge = kt + kRows > N || (p.causal && kt + kRows - 1 > max(wq0, pre - 1));
+    const bool mixed = docs && (id < 0 || id != wid);
+    const bool near = cap && cap_is_near(s, p);
+    // The forward's unmasked tiles take the cap's last product into the exponent, p =
+    // exp2(s f(s) - m), one operation a score less (prefill [1,32:8,8192,128] @K).
+    const bool fused = MODE == 0 && cap && !bias && near && !edge && !mixed;
+    if (cap && !fused) {
+      cap_scores(s, near, p);
+    } else if (bias && !cap) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] *= p.scale_log2;
     }
@@ -570,12 +580,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
     }
     if (bias) add_bias(s, slope2, static_cast<float>(kt + 4 * hi - qrow));
     constexpr float kDead = MODE == 1 ? kDeadScore : -INFINITY;
-    if (kt + kRows > N || (p.causal && kt + kRows - 1 > max(wq0, pre - 1))) {
+    if (edge) {
       const int bound = last - kt - 4 * hi;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) > bound ? kDead : s[r];
     }
-    if (docs && (id < 0 || id != wid)) {
+    if (mixed) {
       if (id >= 0) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = my_id == id ? s[r] : kDead;
@@ -590,12 +600,21 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
       // score outgrew m by more than the slack (always so from m = -1e30).
       constexpr float kRescaleLimit = 256.0f;
       float ls = 0.0f;
+      if (fused) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        pm[r] = fast_exp2(fmaf(s[r], c, -m_run));
-        ls += pm[r];
+        for (int r = 0; r < 16; ++r) {
+          pm[r] = fast_exp2(fmaf(s[r], cap_factor(s[r], p), -m_run));
+          ls += pm[r];
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          pm[r] = fast_exp2(fmaf(s[r], c, -m_run));
+          ls += pm[r];
+        }
       }
       if (__builtin_amdgcn_ballot_w64(!(ls <= kRescaleLimit)) != 0) {
+        if (fused) cap_scores(s, true, p);
         float mx = s[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
@@ -840,7 +859,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu((sizeo
       if constexpr (DO_DK) dp = mma(rd.row(ds, kk), vf[kk], dp);
     }
     if (cap) {
-      cap_scores(s, p);
+      cap_scores(s, cap_is_near(s, p), p);
     } else if (bias) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] *= p.scale_log2;
