@@ -153,10 +153,11 @@ __device__ __forceinline__ void preload_args(const TokenParams& p) {
     asm volatile("" ::"s"(p.k_scale), "s"(p.v_scale), "s"(p.block_table), "s"(p.max_blocks), "s"(p.num_pages), "s"(p.page_shift));
 }
 
-// Registers: 8-bit rows of up to 128 leave room for four waves per SIMD (their tiles
-// are half as large: LDS holds four workgroups).
+// Registers: 8-bit rows of up to 128 leave room for four waves per SIMD, three where D
+// is less than the padded width (their tiles are half as large: LDS holds four
+// workgroups).
 template <int DP, int ROWS, int CACHE>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(CACHE != kF16 && DP <= 128 && ROWS != kRowElems ? 4 : 1))) void token_kernel(
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(CACHE != kF16 && DP <= 128 ? (ROWS == kRowFull ? 4 : (ROWS == kRowChunks ? 3 : 1)) : 1))) void token_kernel(
     TokenParams p) {
   constexpr bool C8 = CACHE != kF16;
   constexpr int ES = C8 ? 1 : 2;
