@@ -190,7 +190,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(CACHE 
     const int per_seq = p.H_KV * p.num_hg;
     // A page's scales lie side by side for all its heads, one line for the units of a
     // sequence: workgroups go to XCD j % 8, and within every whole 64 of them an XCD takes
-    // eight neighbours, so that eight heads share a line in one L2 (@J).
+    // eight neighbours, so that eight heads share a line in one L2 (step of [128] to 4096 keys
+    // 103.4 -> 100.9 us).
     int item = static_cast<int>(blockIdx.x);
     if (C8 && (item | 63) < static_cast<int>(gridDim.x)) item = (item & ~63) | (item & 7) << 3 | (item >> 3 & 7);
     const RaggedItem it = p.B <= 64    ? ragged_item<1>(len, item, p.B, per_seq, p.N, S, kLongChunk, C8)
@@ -787,6 +788,11 @@ static int contiguous(const char* fn, const void* q, const void* k, const void* 
   if (weighted && (reinterpret_cast<uintptr_t>(scores) & 15) != 0)
     return set_error(FA_ERR_INVALID_ARG, "%s: scratch must be 16-byte aligned", fn);
   if (B > 0 && weighted && (!weight || !weight_out || !scores)) return set_error(FA_ERR_INVALID_ARG, "%s: null pointer", fn);
+  // one array, or two apart: in between, a sum would be read as another key's weight
+  const size_t weight_bytes = static_cast<size_t>(B) * H_KV * N * sizeof(float);
+  const uintptr_t w0 = reinterpret_cast<uintptr_t>(weight), w1 = reinterpret_cast<uintptr_t>(weight_out);
+  if (weighted && w0 != w1 && w0 < w1 + weight_bytes && w1 < w0 + weight_bytes)
+    return set_error(FA_ERR_INVALID_ARG, "%s: weight and weight_out overlap in part", fn);
   if (weighted && static_cast<long long>(B) * H_KV > 65535)
     return set_error(FA_ERR_UNSUPPORTED, "%s: more than 65535 (sequence, KV head) pairs", fn);
   TokenParams p = {};

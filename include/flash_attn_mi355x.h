@@ -374,7 +374,7 @@ int fa_decode_scored_fp16(const void* q, const void* k, const void* v, void* o,
  *   weight_out[b, h_kv, t] = weight[b, h_kv, t] + sum over the KV head's query
  *   heads of their softmax weight of key t, for the keys attended; other
  *   entries of weight_out are left as they are.  weight/weight_out fp32 [B,
- *   H_KV, N]; they may be one array.  The scratch holds
+ *   H_KV, N]; they may be one array, and must not overlap otherwise.  The scratch holds
  *   fa_decode_weighted_scratch_size(B, H_Q, N) bytes, 16-byte aligned, and needs no
  *   initialisation.
  *   B * H_KV <= 65535.  Two launches.
@@ -437,7 +437,8 @@ int fa_paged_decode_kv8(const void* q, const void* k_cache,
  *   in their order to the front of k_out/v_out [B, H_KV, capacity, D], their weights
  *   to weight_out and their old positions to index (int32) [B, H_KV, capacity];
  *   rows past them are 0, 0 and -1.  new_lens[b] = min(L, budget).
- *   0 <= recent <= budget <= capacity; B * H_KV <= 65535.  Two launches.
+ *   0 <= recent <= budget <= capacity; B * H_KV <= 65535.  The outputs must not
+ *   overlap the inputs or each other.  Two launches.
  */
 int fa_evict_by_weight(const void* k, const void* v, const float* weight,
                        const int32_t* seq_lens, void* k_out, void* v_out,
