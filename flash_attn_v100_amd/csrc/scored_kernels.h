@@ -274,7 +274,8 @@ constexpr float kDeadScore = -1e15f;
 // polynomial of common.h with the scales folded into its coefficients, y = s (c0 +
 // c1 s^2 + ...): 6 full-rate operations a score, where the exponential form takes two
 // quarter-rate ones and 9 others.  (These kernels are bound by their vector
-// instructions: with the coefficients unfolded, 9 a score, @E.)
+// instructions: with the coefficients unfolded, 9 a score, prefill
+// [1,32:8,8192,128] takes 689 us for 658.)
 __device__ __forceinline__ float cap_factor(float s, const ScoredParams& p) {
   const float w = s * s;
   return fmaf(fmaf(fmaf(fmaf(p.cap_poly[4], w, p.cap_poly[3]), w, p.cap_poly[2]), w, p.cap_poly[1]), w, p.cap_poly[0]);
@@ -302,8 +303,9 @@ __device__ __forceinline__ void add_bias(float16_t& y, float slope2, float rel) 
 }
 
 // Ids of the staged tiles' rows, beside the ring: they travel with the tile, so
-// that a tile of several documents waits for nothing of its own (read from
-// global memory where a tile needs them, they drained the copies in flight: @H).
+// that a tile of several documents waits for nothing of its own.  (Read from global
+// memory where a tile needs them, they drain the copies in flight; measured the same,
+// 116 to 120 us either way for the forward of documents [4,32:8,2048,128].)
 constexpr int kStagedIds = kWaves * kRows;  // rows of a stage, at most
 
 // Fetches the ids of rows [r0, r0 + SR) (past `rows`: the last row's) into a stage's slots.
@@ -455,7 +457,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
   walk.first = 0;
   walk.count = (kend + SR - 1) / SR;
   // With a bias the nearest keys weigh most: a walk that starts at the diagonal
-  // finds the running maximum at once (full [8,16,577,80] @I).  With ids, the
+  // finds the running maximum at once (full [8,16,577,80] 43.6 -> 38.4 us).  With ids, the
   // diagonal tile is sure to be needed.
   walk.rev = p.causal && (bias || docs);
   walk.start = !p.causal && (bias || docs) ? q0 / SR : 0;
@@ -563,7 +565,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
     const bool mixed = docs && (id < 0 || id != wid);
     const bool near = cap && cap_is_near(s, p);
     // The forward's unmasked tiles take the cap's last product into the exponent, p =
-    // exp2(s f(s) - m), one operation a score less (prefill [1,32:8,8192,128] @K).
+    // exp2(s f(s) - m), one operation a score less (prefill [1,32:8,8192,128] 658 -> 649 us).
     const bool fused = MODE == 0 && cap && !bias && near && !edge && !mixed;
     if (cap && !fused) {
       cap_scores(s, near, p);
@@ -720,13 +722,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(query_
 }
 
 // ---------------------------------------------------------------------------
-// Key-major kernel for 32 keys per wave: PASS 0 = dV, 1 = dK, 2 = both.
-constexpr int kPassDV = 0, kPassDK = 1, kPassBoth = 2;
-template <typename T, int DP, int DC, int ROWS, int PASS, int SPLIT, int MODS>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu((sizeof(T) == 4 ? DP <= 64 && SPLIT <= 2 : PASS == kPassBoth && DP == 128 && SPLIT <= 2 && (MODS & kAnyMods) == 0) ? 2 : 1))) void scored_key_kernel(
+// Waves per SIMD that the key kernel's registers leave room for: two where LDS holds two
+// workgroups and the variant is compiled in (both accumulators of 128 fit 256 registers).
+template <typename T, int DP, int SPLIT, int MODS>
+constexpr int key_waves() {
+  if (SPLIT > 2) return 1;
+  return (sizeof(T) == 4 ? DP <= 64 : DP == 128 && (MODS & kAnyMods) == 0) ? 2 : 1;
+}
+
+// Key-major kernel for 32 keys per wave: dV += P^T dO and dK += dS^T Q.
+template <typename T, int DP, int DC, int ROWS, int SPLIT, int MODS>
+__global__ __launch_bounds__(kThreads)
+__attribute__((amdgpu_waves_per_eu(key_waves<T, DP, SPLIT, MODS>()))) void scored_key_kernel(
     ScoredParams p) {
-  constexpr bool DO_DV = PASS != kPassDK;
-  constexpr bool DO_DK = PASS != kPassDV;
   typedef typename Elem<T>::frag F;
   constexpr int KK = DC / 16;
   constexpr int DB = (DC + 31) / 32;
@@ -774,10 +782,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu((sizeo
     const T* qp = static_cast<const T*>(p.q) + head * N * D;
     const T* dp = static_cast<const T*>(p.dout) + head * N * D;
     const float* lse = p.row_lse + head * N;
-    // the dV pass never reads delta: lse stands in for it in its stream
-    const float* second = DO_DK ? p.delta + head * N : lse;
-    if constexpr (DMA) ring.dma(qp, dp, lse, second, qstart + tile * SR, N, D, stage);
-    else ring.load(qp, dp, lse, second, qstart + tile * SR, N, D);
+    const float* delta = p.delta + head * N;
+    if constexpr (DMA) ring.dma(qp, dp, lse, delta, qstart + tile * SR, N, D, stage);
+    else ring.load(qp, dp, lse, delta, qstart + tile * SR, N, D);
     if (docs) fetch_ids<SR, DMA>(walk.ids, qstart + tile * SR, N, s_ids[stage]);
   };
   // every read that the walk waits for, before the first wait
@@ -798,7 +805,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu((sizeo
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       kf[kk] = load_frag<T, ROWS>(static_cast<const T*>(p.k) + row, 16 * kk + 8 * hi, D);
-      if constexpr (DO_DK) vf[kk] = load_frag<T, ROWS>(static_cast<const T*>(p.v) + row, 16 * kk + 8 * hi, D);
+      vf[kk] = load_frag<T, ROWS>(static_cast<const T*>(p.v) + row, 16 * kk + 8 * hi, D);
     }
   }
   if (walk.own) fetch(0, 0, 0);
@@ -822,7 +829,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu((sizeo
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       kf[kk] = zero_frag<T>();
-      if constexpr (DO_DK) vf[kk] = zero_frag<T>();
+      vf[kk] = zero_frag<T>();
     }
   }
   float16_t dk[DB], dv[DB];
@@ -856,7 +863,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu((sizeo
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       s = mma(rd.row(qs, kk), kf[kk], s);
-      if constexpr (DO_DK) dp = mma(rd.row(ds, kk), vf[kk], dp);
+      dp = mma(rd.row(ds, kk), vf[kk], dp);
     }
     if (cap) {
       cap_scores(s, cap_is_near(s, p), p);
@@ -865,7 +872,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu((sizeo
       for (int r = 0; r < 16; ++r) s[r] *= p.scale_log2;
     }
     // derivative of the cap: from the capped score where that is still at hand
-    constexpr bool kKeepDt = DO_DK && (MODS & kAnyMods) != 0;
+    constexpr bool kKeepDt = (MODS & kAnyMods) != 0;
     float16_t dt;
     if constexpr (kKeepDt) {
 #pragma unroll
@@ -894,34 +901,27 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu((sizeo
 #pragma unroll
     for (int rr = 0; rr < 4; ++rr) {
       const float4_t l4 = *reinterpret_cast<const __attribute__((address_space(3))) float4_t*>(lv + 8 * rr + 4 * hi);
-      float4_t d4;
-      if constexpr (DO_DK) d4 = *reinterpret_cast<const __attribute__((address_space(3))) float4_t*>(dvv + 8 * rr + 4 * hi);
+      const float4_t d4 = *reinterpret_cast<const __attribute__((address_space(3))) float4_t*>(dvv + 8 * rr + 4 * hi);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = 4 * rr + j;
         pm[r] = fast_exp2(fmaf(s[r], c, -l4[j]));
-        if constexpr (DO_DK) {
-          dsm[r] = (dp[r] - d4[j]) * pm[r];
-          if constexpr (kKeepDt) dsm[r] *= dt[r];
-          else if (cap) dsm[r] *= fmaf(s[r] * s[r], -p.cap_slope, 1.0f);
-        }
+        dsm[r] = (dp[r] - d4[j]) * pm[r];
+        if constexpr (kKeepDt) dsm[r] *= dt[r];
+        else if (cap) dsm[r] *= fmaf(s[r] * s[r], -p.cap_slope, 1.0f);
       }
     }
-    if constexpr (DO_DV) {
-      const F pf0 = acc_frag<T>(pm, 0), pf1 = acc_frag<T>(pm, 1);
+    const F pf0 = acc_frag<T>(pm, 0), pf1 = acc_frag<T>(pm, 1);
 #pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        dv[db] = mma(rd.tr(ds, 0, db), pf0, dv[db]);
-        dv[db] = mma(rd.tr(ds, 16, db), pf1, dv[db]);
-      }
+    for (int db = 0; db < DB; ++db) {
+      dv[db] = mma(rd.tr(ds, 0, db), pf0, dv[db]);
+      dv[db] = mma(rd.tr(ds, 16, db), pf1, dv[db]);
     }
-    if constexpr (DO_DK) {
-      const F sf0 = acc_frag<T>(dsm, 0), sf1 = acc_frag<T>(dsm, 1);
+    const F sf0 = acc_frag<T>(dsm, 0), sf1 = acc_frag<T>(dsm, 1);
 #pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        dk[db] = mma(rd.tr(qs, 0, db), sf0, dk[db]);
-        dk[db] = mma(rd.tr(qs, 16, db), sf1, dk[db]);
-      }
+    for (int db = 0; db < DB; ++db) {
+      dk[db] = mma(rd.tr(qs, 0, db), sf0, dk[db]);
+      dk[db] = mma(rd.tr(qs, 16, db), sf1, dk[db]);
     }
   });
 
@@ -950,8 +950,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu((sizeo
         }
       }
     };
-    if constexpr (DO_DV) join(dv);
-    if constexpr (DO_DK) join(dk);
+    join(dv);
+    join(dk);
     if (sub > 0) return;
   }
 
@@ -965,8 +965,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu((sizeo
       const int d0 = 32 * db + 8 * rr + 4 * hi;
       auto x = [&](int j) { return dk[db][4 * rr + j] * p.scale; };
       auto y = [&](int j) { return dv[db][4 * rr + j]; };
-      if constexpr (DO_DK) store4<T, ROWS>(dkp, d0, D, x(0), x(1), x(2), x(3));
-      if constexpr (DO_DV) store4<T, ROWS>(dvp, d0, D, y(0), y(1), y(2), y(3));
+      store4<T, ROWS>(dkp, d0, D, x(0), x(1), x(2), x(3));
+      store4<T, ROWS>(dvp, d0, D, y(0), y(1), y(2), y(3));
     }
 }
 

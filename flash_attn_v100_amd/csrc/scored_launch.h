@@ -69,13 +69,13 @@ void launch_query(ScoredParams p, int split, hipStream_t st) {
   });
 }
 
-template <typename T, int DP, int DC, int ROWS, int PASS, int MODS>
+template <typename T, int DP, int DC, int ROWS, int MODS>
 void launch_key(ScoredParams p, int split, hipStream_t st) {
   by_split<T, DP, ROWS>(split, [&](auto s) {
     p.nblk = ceil_div(p.N, kBlockRows / s());
     const long long blocks = deal(p, static_cast<long long>(p.B) * p.H_KV, 1);
     p.snake = snake_order(p, blocks, true);
-    hipLaunchKernelGGL((scored_key_kernel<T, DP, DC, ROWS, PASS, s(), MODS>), dim3(static_cast<unsigned>(blocks)),
+    hipLaunchKernelGGL((scored_key_kernel<T, DP, DC, ROWS, s(), MODS>), dim3(static_cast<unsigned>(blocks)),
                        dim3(kThreads), 0, st, p);
   });
 }
@@ -97,18 +97,13 @@ inline int split_key(const ScoredParams& p) {
 template <typename T, int DP, int DC, int ROWS, int MODS>
 void launch_backward_shape(const ScoredParams& p, hipStream_t st) {
   launch_query<T, DP, DC, ROWS, 1, MODS>(p, split_query(p, true), st);
-  if constexpr (sizeof(T) == 2 && DP > 64 && false) {
-    launch_key<T, DP, DC, ROWS, kPassDV, MODS>(p, split_key(p), st);
-    launch_key<T, DP, DC, ROWS, kPassDK, MODS>(p, split_key(p), st);
-  } else {
-    launch_key<T, DP, DC, ROWS, kPassBoth, MODS>(p, split_key(p), st);
-  }
+  launch_key<T, DP, DC, ROWS, MODS>(p, split_key(p), st);
 }
 
 // Calls run with the variant of the call's modifications: those met in practice
 // have one of their own, what is left reads them from the parameters.
-// Compiled in, prefill [1,32:8,8192,128] with a cap takes @A us for @B, a training
-// layer of documents [4,32:8,2048,128] @C for @D.
+// Compiled in, prefill [1,32:8,8192,128] with a cap takes 658 us for 690, a training
+// layer of documents [4,32:8,2048,128] 495 for 633.
 template <typename Run>
 void by_mods(int mods, Run&& run) {
   switch (mods) {
