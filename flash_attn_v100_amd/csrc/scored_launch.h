@@ -82,7 +82,11 @@ void launch_key(ScoredParams p, int split, hipStream_t st) {
 
 // Waves that share a row block (each walks 1 / split of its tiles), by the 128-row
 // blocks of the call: few blocks leave CUs idle or with little to switch to, and are
-// bound by the longest walk.
+// bound by the longest walk.  Four against one, 16 blocks, [1,8,256,64]: forward 6.7 us
+// for 10.4, dQ 7.7 for 13.0, key kernel 7.8 for 13.3; the fp32 step [2,16,1000,64], 256
+// blocks, 242 for 392.  With enough blocks the split only adds its join: prefill
+// [8,16,577,80], 640 blocks, 38.5 unsplit, 53.3 in two.  The key kernel at 512 blocks
+// (documents [4,32:8,2048,128]): in two 248, unsplit 314.
 inline int split_query(const ScoredParams& p, bool backward) {
   const long long blocks = static_cast<long long>(p.B) * p.H_Q * ceil_div(p.N, kBlockRows);
   if (blocks <= 64) return 4;
